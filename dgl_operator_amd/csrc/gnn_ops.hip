@@ -363,8 +363,9 @@ at::Tensor sddmm_dot(at::Tensor src, at::Tensor dst, at::Tensor feat_u,
   const int64_t E = src.numel();
   int H = 1, D = fu.size(-1);
   if (fu.dim() == 3) H = fu.size(1);
-  at::Tensor out = (H == 1) ? at::empty({E}, fu.options())
-                            : at::empty({E, H}, fu.options());
+  // [N, H, D] -> [E, H] for one head too, as on the CPU
+  at::Tensor out = (fu.dim() != 3) ? at::empty({E}, fu.options())
+                                   : at::empty({E, H}, fu.options());
   const int block = 256;
   const int grid = grid_for(E * H, block);
   auto stream = cur_stream();

@@ -69,6 +69,12 @@ def spmm_raw(
     return _spmm_ref(indptr, indices, feat, eweight, mean)
 
 
+def _weight_shaped(grad_w: torch.Tensor, eweight: torch.Tensor) -> torch.Tensor:
+    """One head's [E, 1] for scalar weights [E], and the other way round."""
+    return (grad_w.view_as(eweight) if grad_w.numel() == eweight.numel()
+            else grad_w)
+
+
 class _GSpMM(torch.autograd.Function):
     """copy_u/u_mul_e + sum/mean with autograd through feat and eweight.
 
@@ -113,7 +119,8 @@ class _GSpMM(torch.autograd.Function):
                 from .sddmm import sddmm_dot_raw
 
                 dst = _edge_dst(cindptr)
-                grad_w = sddmm_dot_raw(cindices, dst, feat, grad_out)
+                grad_w = _weight_shaped(
+                    sddmm_dot_raw(cindices, dst, feat, grad_out), eweight)
             return None, grad_feat, grad_w, None
         rindptr, rindices, reids = gstruct.csr()
         if ctx.needs_input_grad[1]:
@@ -132,7 +139,8 @@ class _GSpMM(torch.autograd.Function):
             from .sddmm import sddmm_dot_raw
 
             dst = _edge_dst(cindptr)
-            grad_w = sddmm_dot_raw(cindices, dst, feat, grad_out)
+            grad_w = _weight_shaped(
+                sddmm_dot_raw(cindices, dst, feat, grad_out), eweight)
         return None, grad_feat, grad_w, None
 
 

@@ -417,7 +417,8 @@ def main():
                   "eager stepping")
             opt = torch.optim.Adam(model.parameters(), lr=args.lr)
 
-    use_prefetch = prefetch_ok and not use_capture
+    # a forced capture (--capture) that fails steps plainly, as its message says
+    use_prefetch = prefetch_ok and not use_capture and args.capture is not True
     if use_prefetch:
         base_step = one_step
         one_step = _make_prefetched_step(base_step)

@@ -192,6 +192,10 @@ class Manager:
                 self._written_statuses.pop(key, None)
             elif self.watch_crs:
                 self._write_status(job)
+            # the lease is good for a ttl from its renewal: a pass that takes
+            # longer (many kubectl calls a job) must not let a standby in
+            if not self._ensure_leadership():
+                return
 
     def run(self, metrics_port: Optional[int] = None,
             health_port: Optional[int] = None, block: bool = True):

@@ -25,6 +25,9 @@ SOURCES = [
     "adagrad.hip",
     "kge.hip",
     "gather_mm.hip",
+    "route.hip",
+    "segment_mm.hip",
+    "log_probs.hip",
     "ldg.cpp",
     "bindings.cpp",
 ]
@@ -42,7 +45,7 @@ def _torch_paths():
 def _needs_build(obj: Path, src: Path) -> bool:
     if not obj.exists():
         return True
-    deps = [src, CSRC / "common.h", CSRC / "build.py"]
+    deps = [src, CSRC / "common.h", CSRC / "vec.h", CSRC / "build.py"]
     return any(d.exists() and d.stat().st_mtime > obj.stat().st_mtime for d in deps)
 
 

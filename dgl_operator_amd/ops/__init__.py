@@ -12,6 +12,9 @@ from .sampling import (
 from .kge import get_score_func, kge_loss, SCORE_FUNCS
 from .adagrad import sparse_adagrad_update
 from .gather_mm import gather_mm, GatherView
+from .route import RowRoute, route_rows, dispatch_rows, combine_rows
+from .segment_mm import segment_mm
+from .log_probs import LogProbs, log_probs
 
 __all__ = [
     "backend",
@@ -34,4 +37,11 @@ __all__ = [
     "sparse_adagrad_update",
     "gather_mm",
     "GatherView",
+    "RowRoute",
+    "route_rows",
+    "dispatch_rows",
+    "combine_rows",
+    "segment_mm",
+    "LogProbs",
+    "log_probs",
 ]

@@ -1,0 +1,93 @@
+"""Product of each group of rows with its own weight (typed / expert product).
+
+``segment_mm(offsets, x, weight)`` is y[r] = x[r] @ weight[g] for the rows
+offsets[g]..offsets[g+1] of every group g, the layout ``route_rows`` and
+``segment_reduce`` use: relation-typed projections, heterogeneous layers, a
+mixture's experts. GPU: hand-written MFMA kernels (csrc/segment_mm.hip), one
+launch whatever the groups' sizes, no host synchronisation; CPU: plain PyTorch.
+"""
+from __future__ import annotations
+
+import torch
+from torch.autograd.function import once_differentiable
+
+from . import backend
+
+
+def _bounds(offsets: torch.Tensor, rows: int):
+    ends = offsets.clamp(0, rows).tolist()
+    return [(g, a, b) for g, (a, b) in enumerate(zip(ends[:-1], ends[1:]))
+            if a < b]
+
+
+def _wide(t: torch.Tensor) -> torch.Tensor:
+    return t if t.dtype == torch.float64 else t.float()
+
+
+def _segment_mm_ref(offsets, x, weight):
+    y = x.new_zeros((x.shape[0], weight.shape[2]))
+    for g, a, b in _bounds(offsets, x.shape[0]):
+        y[a:b] = (_wide(x[a:b]) @ _wide(weight[g])).to(y.dtype)
+    return y
+
+
+class _SegmentMM(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, offsets, x, weight):
+        need_x, need_w = ctx.needs_input_grad[1:]
+        ctx.save_for_backward(offsets, x if need_w else None,
+                              weight if need_x else None)
+        if x.is_cuda:
+            ext = backend.ext_for(x)
+            return ext.segment_mm(offsets, x, weight, False)
+        return _segment_mm_ref(offsets, x, weight)
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, grad_out):
+        offsets, x, weight = ctx.saved_tensors
+        need_x, need_w = ctx.needs_input_grad[1:]
+        dx = dw = None
+        if grad_out.is_cuda:
+            ext = backend.ext_for(grad_out)
+            if need_x:
+                dx = ext.segment_mm(offsets, grad_out, weight, True)
+            if need_w:
+                dw = ext.segment_mm_wgrad(offsets, x, grad_out)
+        else:
+            if need_x:
+                dx = _segment_mm_ref(offsets, grad_out, weight.transpose(1, 2))
+            if need_w:
+                dw = x.new_zeros((offsets.numel() - 1, x.shape[1],
+                                  grad_out.shape[1]))
+                for g, a, b in _bounds(offsets, x.shape[0]):
+                    dw[g] = (_wide(x[a:b]).t() @ _wide(grad_out[a:b])
+                             ).to(dw.dtype)
+        return None, dx, dw
+
+
+def segment_mm(offsets: torch.Tensor, x: torch.Tensor,
+               weight: torch.Tensor) -> torch.Tensor:
+    """y[r] = x[r] @ weight[g] for offsets[g] <= r < offsets[g+1].
+
+    offsets  int64 [groups + 1], not falling, within [0, rows]
+    x        [rows, K] fp32, bf16 or fp16 (fp64 on CPU too), any row stride
+    weight   [groups, K, N] of the same type, any strides (a transposed view of
+             [groups, N, K] is read in place)
+
+    Groups may be empty; rows of no group give zeros. Products accumulate in
+    fp32 and are rounded once. Gradients reach x and weight.
+    """
+    assert offsets.dim() == 1 and offsets.dtype == torch.int64, \
+        "segment_mm: int64 offsets [groups + 1] expected"
+    assert x.dim() == 2 and weight.dim() == 3, \
+        "segment_mm: x [rows, K] and weight [groups, K, N] expected"
+    assert weight.shape[0] >= 1 and offsets.numel() == weight.shape[0] + 1, \
+        f"segment_mm: {weight.shape[0]} weights need {weight.shape[0] + 1} offsets"
+    assert x.shape[1] == weight.shape[1], \
+        f"segment_mm: rows of {x.shape[1]} by weights of {weight.shape[1]}"
+    assert x.dtype == weight.dtype and x.is_floating_point(), \
+        "segment_mm: x and weight must share a floating point type"
+    assert x.device == weight.device == offsets.device, \
+        "segment_mm: all tensors must be on one device"
+    return _SegmentMM.apply(offsets.contiguous(), x, weight)

@@ -30,111 +30,563 @@ __device__ inline float key_value(uint64_t k) {
   return __uint_as_float((b & 0x80000000u) ? (b & 0x7fffffffu) : ~b);
 }
 
-template <typename F, typename Op>
-__device__ inline F block_reduce(F v, F* tmp, Op op) {
-#pragma unroll
-  for (int d = 1; d < 64; d <<= 1) v = op(v, __shfl_xor(v, d));
-  __syncthreads();
-  if ((threadIdx.x & 63) == 0) tmp[threadIdx.x >> 6] = v;
-  __syncthreads();
-  v = tmp[0];
-  for (int w = 1; w < (int)(blockDim.x >> 6); ++w) v = op(v, tmp[w]);
-  return v;
-}
-
-template <typename T>
-__global__ __launch_bounds__(256) void log_probs_kernel(
-    const T* __restrict__ z, int64_t zs, const int64_t* __restrict__ target,
-    int64_t ignore, int C, int k, float* __restrict__ lp,
-    float* __restrict__ ent, float* __restrict__ top_lp,
-    int64_t* __restrict__ top_idx, float* __restrict__ stats) {
-  __shared__ float tmp[4];
-  __shared__ uint64_t ktmp[4];
-  const int64_t row = blockIdx.x;
-  const T* zr = z + row * zs;
-  float m = -INFINITY;
-  for (int j = threadIdx.x; j < C; j += 256) m = fmaxf(m, (float)zr[j]);
-  m = block_reduce(m, tmp, [](float a, float b) { return fmaxf(a, b); });
-  const float base = m == -INFINITY ? 0.f : m;
-  float s = 0.f, a = 0.f;
-  for (int j = threadIdx.x; j < C; j += 256) {
-    const float d = (float)zr[j] - base;
-    const float e = __expf(d);
-    s += e;
-    a += fmaxf(d, -1e30f) * e;  // -inf * 0
+// what a row's sums say
+struct RowStat {
+  float base, logs;
+  bool none;
+  __device__ RowStat(float m, float s) {
+    none = s == 0.f;
+    base = m == -INFINITY ? 0.f : m;
+    logs = none ? 0.f : logf(s);
   }
-  s = block_reduce(s, tmp, [](float x, float y) { return x + y; });
-  a = block_reduce(a, tmp, [](float x, float y) { return x + y; });
-  const bool none = s == 0.f;
-  const float logs = none ? 0.f : logf(s);
-  if (threadIdx.x == 0) {
+  __device__ float log_p(float z) const { return (z - base) - logs; }
+  __device__ void write(int64_t row, float a, float s, float* ent,
+                        float* stats) const {
     ent[row] = none ? 0.f : logs - a / s;
     stats[2 * row] = base;
     stats[2 * row + 1] = none ? INFINITY : logs;  // the mark of an empty row
-    if (target) {
-      const int64_t t = target[row];
-      float v = NAN;
-      if (t == ignore) v = 0.f;
-      else if (t >= 0 && t < C)
-        v = none ? -INFINITY : ((float)zr[t] - base) - logs;
-      lp[row] = v;
+  }
+  __device__ float answer(float z) const { return none ? -INFINITY : log_p(z); }
+};
+
+// one term of s and a; -inf is 0 in both, NaN spoils both
+__device__ inline void add_term(float z, float base, float& s, float& a) {
+  const float d = z - base;
+  const float e = __expf(d);
+  s += e;
+  a += fmaxf(d, -1e30f) * e;
+}
+
+template <typename T>
+__device__ inline void write_answer(const T* zr, const RowStat& st, int64_t row,
+                                    const int64_t* target, int64_t ignore,
+                                    int C, float* lp) {
+  const int64_t t = target[row];
+  lp[row] = t == ignore ? 0.f
+                        : (t >= 0 && t < C) ? st.answer((float)zr[t]) : NAN;
+}
+
+// ---------------------------------------------------------------------------
+// Short rows: L lanes a row, 64 / L rows a wave. A wave copies its rows to LDS
+// (16 bytes a lane, whatever the rows' alignment), each lane walks its part of
+// one row and keeps the K best keys sorted in registers: an insertion is one
+// median a slot for 16-bit logits, whose value and index fit one word.
+// Lanes start at different places of their rows where an even length would
+// send them to the same banks; the keys hold the index, so order is free.
+// ---------------------------------------------------------------------------
+template <typename T>
+struct SmallKey;
+template <>
+struct SmallKey<float> {
+  using type = uint64_t;
+  static __device__ uint64_t make(float z, int j) { return top_key(z, j); }
+  static __device__ int index(uint64_t k) { return key_index(k); }
+  static __device__ float value(uint64_t k) { return key_value(k); }
+  // x into the falling list; the last one drops out
+  template <int K>
+  static __device__ void insert(uint64_t (&list)[K], uint64_t x) {
+#pragma unroll
+    for (int i = 0; i < K; ++i) {
+      const uint64_t o = list[i];
+      const bool c = x > o;
+      list[i] = c ? x : o;
+      x = c ? o : x;
     }
   }
+};
+template <typename T>
+struct SmallKey {  // 16-bit types: the index has 16 bits too
+  using type = uint32_t;
+  static __device__ uint32_t make(T v, int j) {
+    uint32_t b = __builtin_bit_cast(uint16_t, v);
+    if ((b & 0x7fffu) == 0) b = 0;
+    if (v != v) b = 0x7fffu;
+    b = (b & 0x8000u) ? ~b & 0xffffu : b | 0x8000u;
+    return b << 16 | (0xffffu - j);
+  }
+  static __device__ int index(uint32_t k) { return 0xffff - (k & 0xffffu); }
+  static __device__ float value(uint32_t k) {
+    const uint32_t b = k >> 16;
+    return (float)__builtin_bit_cast(
+        T, (uint16_t)((b & 0x8000u) ? b & 0x7fffu : ~b));
+  }
+  template <int K>
+  static __device__ void insert(uint32_t (&list)[K], uint32_t x) {
+#pragma unroll
+    for (int i = K - 1; i > 0; --i) {  // median of x and two neighbours
+      const uint32_t hi = list[i - 1], lo = list[i];
+      list[i] = max(min(hi, lo), min(max(hi, lo), x));
+    }
+    list[0] = max(list[0], x);
+  }
+};
+
+template <typename K>
+__device__ inline K shuffle_key(K k, int d) {
+  if constexpr (sizeof(K) == 4) return __shfl_xor((int)k, d);
+  else return (K)__shfl_xor((unsigned long long)k, d);
+}
+
+template <typename T, int L, int K>
+__global__ __launch_bounds__(256) void log_probs_short_kernel(
+    const T* __restrict__ z, int64_t zs, const int64_t* __restrict__ target,
+    int64_t ignore, int64_t rows, int C, int k, float* __restrict__ lp,
+    float* __restrict__ ent, float* __restrict__ top_lp,
+    int64_t* __restrict__ top_idx, float* __restrict__ stats, int wave_bytes) {
+  extern __shared__ __align__(16) char lds[];
+  constexpr int RW = 64 / L;  // rows a wave
+  using Key = SmallKey<T>;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int64_t row0 = ((int64_t)blockIdx.x * 4 + wave) * RW;
+  if (row0 >= rows) return;
+  char* mine = lds + wave * wave_bytes;
+  T* tile = reinterpret_cast<T*>(mine);
+  const int many = (int)min((int64_t)RW, rows - row0);
+  const T* src = z + row0 * zs;
+  if (zs == C) {
+    constexpr int E = 16 / sizeof(T);
+    const int n = many * C, whole = n / E;
+    for (int i = lane; i < whole; i += 64)
+      reinterpret_cast<Chunk*>(mine)[i] =
+          *reinterpret_cast<const LooseChunk*>(src + i * E);
+    for (int i = whole * E + lane; i < n; i += 64) tile[i] = src[i];
+  } else {
+    for (int r = 0; r < many; ++r)
+      for (int j = lane; j < C; j += 64) tile[r * C + j] = src[r * zs + j];
+  }
+  wave_sync();
+  const int r = lane / L, part = lane % L;
+  const bool live = r < many;
+  const T* zr = tile + (live ? r : 0) * C;
+  // my elements: part, part + L, ... begun at a place of my own
+  const int count = (C - part + L - 1) / L;
+  int begin = (C & 1) || count < 1 ? 0 : r % count;
+  typename Key::type best[K > 0 ? K : 1];
+#pragma unroll
+  for (int i = 0; i < (K > 0 ? K : 1); ++i) best[i] = 0;
+  float m = -INFINITY;
+  for (int i = 0, at = begin; i < count; ++i) {
+    const int j = at * L + part;
+    const T v = zr[j];
+    if constexpr (K > 0) Key::template insert<K>(best, Key::make(v, j));
+    else m = fmaxf(m, (float)v);
+    if (++at == count) at = 0;
+  }
+  if constexpr (K > 0) {
+#pragma unroll
+    for (int d = 1; d < L; d <<= 1) {
+      typename Key::type other[K];
+#pragma unroll
+      for (int i = 0; i < K; ++i) other[i] = shuffle_key(best[i], d);
+      if constexpr ((K & (K - 1)) == 0) {
+        // one list against the other turned round leaves the K best, first
+        // rising then falling: log K exchanges sort them
+#pragma unroll
+        for (int i = 0; i < K; ++i) best[i] = max(best[i], other[K - 1 - i]);
+#pragma unroll
+        for (int h = K / 2; h > 0; h /= 2)
+#pragma unroll
+          for (int i = 0; i < K; ++i)
+            if (!(i & h)) {
+              const auto x = best[i], y = best[i + h];
+              best[i] = max(x, y);
+              best[i + h] = min(x, y);
+            }
+      } else {
+#pragma unroll
+        for (int i = 0; i < K; ++i) Key::template insert<K>(best, other[i]);
+      }
+    }
+    m = Key::value(best[0]);
+  } else {
+#pragma unroll
+    for (int d = 1; d < L; d <<= 1) m = fmaxf(m, __shfl_xor(m, d));
+  }
+  const float base = m == -INFINITY ? 0.f : m;
+  float s = 0.f, a = 0.f;
+  for (int i = 0, at = begin; i < count; ++i) {
+    add_term((float)zr[at * L + part], base, s, a);
+    if (++at == count) at = 0;
+  }
+#pragma unroll
+  for (int d = 1; d < L; d <<= 1) {
+    s += __shfl_xor(s, d);
+    a += __shfl_xor(a, d);
+  }
+  if (!live || part != 0) return;
+  const int64_t row = row0 + r;
+  const RowStat st(m, s);
+  st.write(row, a, s, ent, stats);
+  if (target) write_answer(zr, st, row, target, ignore, C, lp);
+  if constexpr (K > 0) {
+#pragma unroll
+    for (int i = 0; i < K; ++i)
+      if (i < k) {
+        top_idx[row * k + i] = Key::index(best[i]);
+        top_lp[row * k + i] = st.log_p(Key::value(best[i]));
+      }
+  }
+}
+
+// ---------------------------------------------------------------------------
+// Long rows: a block holds up to 16 logits a thread in registers and reads
+// them once; rows longer than that are split over blocks and joined.
+//
+// The best k: the 64 lanes' maxima (over the block's waves) give a threshold,
+// the k-th largest of them, that at least k logits reach; what reaches it is
+// collected (about k of them) and ranked by counting. Where ties or masks let
+// too many through, k rounds of a block maximum find them one by one.
+// ---------------------------------------------------------------------------
+constexpr int kPer = 16;    // logits a thread
+constexpr int kCap = 512;   // collected candidates
+
+template <int NT>
+struct LongShared {
+  float lane_max[NT / 64][64];
+  float sums[2][NT / 64];
+  uint64_t keys[kCap];
+  uint64_t round[NT / 64];
+  float threshold;
+  int count;
+};
+
+// the k largest of the block's keys, falling, each given to emit(rank, key)
+template <int NT, typename Emit>
+__device__ inline void best_of_block(const float (&v)[kPer], int first, int c1,
+                                     const int (&index)[kPer], int k,
+                                     LongShared<NT>& sh, Emit emit) {
+  const float t = sh.threshold;
+#pragma unroll
+  for (int i = 0; i < kPer; ++i)
+    if (!(v[i] < t) && index[i] < c1) {
+      const int at = atomicAdd(&sh.count, 1);
+      if (at < kCap) sh.keys[at] = top_key(v[i], index[i]);
+    }
+  __syncthreads();
+  const int count = sh.count;
+  if (count <= kCap) {
+    for (int i = threadIdx.x; i < count; i += NT) {
+      const uint64_t key = sh.keys[i];
+      int rank = 0;
+      for (int j = 0; j < count; ++j) rank += sh.keys[j] > key;
+      if (rank < k) emit(rank, key);
+    }
+    // fewer than k logits in this part of the row
+    for (int i = count + threadIdx.x; i < k; i += NT) emit(i, 0);
+    return;
+  }
   uint64_t last = ~0ull;
-  for (int i = 0; i < k; ++i) {
+  for (int r = 0; r < k; ++r) {
     uint64_t best = 0;
-    for (int j = threadIdx.x; j < C; j += 256) {
-      const uint64_t key = top_key((float)zr[j], j);
-      if (key < last && key > best) best = key;
+#pragma unroll
+    for (int i = 0; i < kPer; ++i)
+      if (index[i] < c1) {
+        const uint64_t key = top_key(v[i], index[i]);
+        if (key < last && key > best) best = key;
+      }
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) {
+      const uint64_t o = shuffle_key(best, d);
+      best = o > best ? o : best;
     }
-    best = block_reduce(best, ktmp, [](uint64_t x, uint64_t y) {
-      return x > y ? x : y;
-    });
-    if (threadIdx.x == 0) {
-      top_idx[row * k + i] = key_index(best);
-      top_lp[row * k + i] = (key_value(best) - base) - logs;
-    }
+    __syncthreads();
+    if ((threadIdx.x & 63) == 0) sh.round[threadIdx.x >> 6] = best;
+    __syncthreads();
+    for (int w = 0; w < NT / 64; ++w) best = max(best, sh.round[w]);
+    if (threadIdx.x == 0) emit(r, best);
     last = best;
   }
 }
 
+// the value that k of a wave's 64 values reach (-inf: fewer than k are above)
+__device__ inline float kth_of_wave(float v, int k) {
+  int reach = 0;
+#pragma unroll
+  for (int i = 0; i < 64; ++i) {
+    const float o = __uint_as_float(
+        __builtin_amdgcn_readlane(__float_as_uint(v), i));
+    reach += o >= v;
+  }
+  float t = reach >= k ? v : -INFINITY;
+#pragma unroll
+  for (int d = 1; d < 64; d <<= 1) t = fmaxf(t, __shfl_xor(t, d));
+  return t;
+}
+
+template <typename T, int NT>
+__global__ __launch_bounds__(NT) void log_probs_long_kernel(
+    const T* __restrict__ z, int64_t zs, const int64_t* __restrict__ target,
+    int64_t ignore, int C, int k, int splits, int chunk,
+    float* __restrict__ lp, float* __restrict__ ent,
+    float* __restrict__ top_lp, int64_t* __restrict__ top_idx,
+    float* __restrict__ stats, float* __restrict__ part_sums,
+    uint64_t* __restrict__ part_keys) {
+  __shared__ LongShared<NT> sh;
+  constexpr int E = 16 / sizeof(T);
+  const int64_t row = blockIdx.x / splits;
+  const int part = blockIdx.x % splits;
+  const int c0 = part * chunk, c1 = min(C, c0 + chunk);
+  const T* zr = z + row * zs;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  float v[kPer];
+  int index[kPer];
+  float m = -INFINITY;
+#pragma unroll
+  for (int i = 0; i < kPer / E; ++i) {
+    const int j = c0 + (i * NT + threadIdx.x) * E;
+    union { Chunk q; T e[E]; } u;
+    if (j + E <= c1) {
+      u.q = *reinterpret_cast<const LooseChunk*>(zr + j);
+    } else {
+#pragma unroll
+      for (int e = 0; e < E; ++e)
+        u.e[e] = j + e < c1 ? zr[j + e] : (T)-INFINITY;
+    }
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+      v[i * E + e] = (float)u.e[e];
+      index[i * E + e] = j + e;
+      m = fmaxf(m, v[i * E + e]);
+    }
+  }
+  sh.lane_max[wave][lane] = m;
+  if (threadIdx.x == 0) sh.count = 0;
+  __syncthreads();
+#pragma unroll
+  for (int w = 0; w < NT / 64; ++w) m = fmaxf(m, sh.lane_max[w][lane]);
+  if (k > 0 && wave == 0) {
+    const float t = kth_of_wave(m, k);
+    if (lane == 0) sh.threshold = t;
+  }
+#pragma unroll
+  for (int d = 1; d < 64; d <<= 1) m = fmaxf(m, __shfl_xor(m, d));
+  const float base = m == -INFINITY ? 0.f : m;
+  float s = 0.f, a = 0.f;
+#pragma unroll
+  for (int i = 0; i < kPer; ++i) add_term(v[i], base, s, a);
+#pragma unroll
+  for (int d = 1; d < 64; d <<= 1) {
+    s += __shfl_xor(s, d);
+    a += __shfl_xor(a, d);
+  }
+  if (lane == 0) {
+    sh.sums[0][wave] = s;
+    sh.sums[1][wave] = a;
+  }
+  __syncthreads();
+  s = a = 0.f;
+#pragma unroll
+  for (int w = 0; w < NT / 64; ++w) {
+    s += sh.sums[0][w];
+    a += sh.sums[1][w];
+  }
+  if (splits > 1) {
+    if (threadIdx.x == 0) {
+      float* o = part_sums + (int64_t)blockIdx.x * 3;
+      o[0] = m;
+      o[1] = s;
+      o[2] = a;
+    }
+    if (k > 0)
+      best_of_block<NT>(v, c0, c1, index, k, sh, [&](int r, uint64_t key) {
+        part_keys[(int64_t)blockIdx.x * k + r] = key;
+      });
+    return;
+  }
+  const RowStat st(m, s);
+  if (threadIdx.x == 0) {
+    st.write(row, a, s, ent, stats);
+    if (target) write_answer(zr, st, row, target, ignore, C, lp);
+  }
+  if (k > 0)
+    best_of_block<NT>(v, c0, c1, index, k, sh, [&](int r, uint64_t key) {
+      top_idx[row * k + r] = key_index(key);
+      top_lp[row * k + r] = st.log_p(key_value(key));
+    });
+}
+
+// the parts of one row joined: a block a row
+template <typename T>
+__global__ __launch_bounds__(256) void log_probs_join_kernel(
+    const T* __restrict__ z, int64_t zs, const int64_t* __restrict__ target,
+    int64_t ignore, int C, int k, int splits,
+    const float* __restrict__ part_sums, const uint64_t* __restrict__ part_keys,
+    float* __restrict__ lp, float* __restrict__ ent,
+    float* __restrict__ top_lp, int64_t* __restrict__ top_idx,
+    float* __restrict__ stats) {
+  __shared__ uint64_t keys[kCap], round[4];
+  __shared__ float tmp[4];
+  const int64_t row = blockIdx.x;
+  const float* ps = part_sums + row * splits * 3;
+  auto over_block = [&](float v, auto op) {
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) v = op(v, __shfl_xor(v, d));
+    __syncthreads();
+    if ((threadIdx.x & 63) == 0) tmp[threadIdx.x >> 6] = v;
+    __syncthreads();
+    return op(op(tmp[0], tmp[1]), op(tmp[2], tmp[3]));
+  };
+  float m = -INFINITY;
+  for (int p = threadIdx.x; p < splits; p += 256) m = fmaxf(m, ps[3 * p]);
+  m = over_block(m, [](float x, float y) { return fmaxf(x, y); });
+  const float base = m == -INFINITY ? 0.f : m;
+  float s = 0.f, a = 0.f;
+  for (int p = threadIdx.x; p < splits; p += 256) {
+    // sums over a base of their own: e^(z - m_p) -> e^(z - m)
+    const float mp = ps[3 * p];
+    const float d = (mp == -INFINITY ? 0.f : mp) - base;
+    const float e = ps[3 * p + 1] == 0.f ? 0.f : __expf(d);
+    s += ps[3 * p + 1] * e;
+    a += (ps[3 * p + 2] + d * ps[3 * p + 1]) * e;
+  }
+  s = over_block(s, [](float x, float y) { return x + y; });
+  a = over_block(a, [](float x, float y) { return x + y; });
+  const RowStat st(m, s);
+  if (threadIdx.x == 0) {
+    st.write(row, a, s, ent, stats);
+    if (target) write_answer(z + row * zs, st, row, target, ignore, C, lp);
+  }
+  const uint64_t* pk = part_keys + row * splits * k;
+  const int64_t count = (int64_t)splits * k;
+  auto emit = [&](int r, uint64_t key) {
+    top_idx[row * k + r] = key_index(key);
+    top_lp[row * k + r] = st.log_p(key_value(key));
+  };
+  if (count <= kCap) {
+    for (int i = threadIdx.x; i < count; i += 256) keys[i] = pk[i];
+    __syncthreads();
+    for (int i = threadIdx.x; i < count; i += 256) {
+      const uint64_t key = keys[i];
+      int rank = 0;
+      for (int j = 0; j < count; ++j) rank += keys[j] > key;
+      if (key && rank < k) emit(rank, key);
+    }
+    return;
+  }
+  uint64_t last = ~0ull;
+  for (int r = 0; r < k; ++r) {
+    uint64_t best = 0;
+    for (int64_t i = threadIdx.x; i < count; i += 256) {
+      const uint64_t key = pk[i];
+      if (key < last && key > best) best = key;
+    }
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) {
+      const uint64_t o = shuffle_key(best, d);
+      best = o > best ? o : best;
+    }
+    __syncthreads();
+    if ((threadIdx.x & 63) == 0) round[threadIdx.x >> 6] = best;
+    __syncthreads();
+    for (int w = 0; w < 4; ++w) best = max(best, round[w]);
+    if (threadIdx.x == 0) emit(r, best);
+    last = best;
+  }
+}
+
+// ---------------------------------------------------------------------------
 // dz_j = g_lp [j = t] + sum_i g_i [j = idx_i]
 //        - p_j (g_lp + sum_i g_i + g_H (log p_j + H))
+// A block makes a tile in LDS, in fp32: several whole rows or a part of a long
+// one. The common term comes first, then the alternatives' own (different
+// places), then the target's, and the tile is rounded once on its way out.
+// ---------------------------------------------------------------------------
+constexpr int kTileElems = 4096;
+constexpr int kTileRows = 64;
+
+struct RowPull {
+  float base, logs, pull, gh, ent;
+};
+
 template <typename T>
 __global__ __launch_bounds__(256) void log_probs_bwd_kernel(
     const T* __restrict__ z, int64_t zs, const int64_t* __restrict__ target,
     int64_t ignore, const int64_t* __restrict__ top_idx,
     const float* __restrict__ stats, const float* __restrict__ ent,
     const float* __restrict__ g_lp, const float* __restrict__ g_ent,
-    const float* __restrict__ g_top, int C, int k, T* __restrict__ dz) {
-  const int64_t row = blockIdx.x;
-  const T* zr = z + row * zs;
-  T* out = dz + row * C;
-  const float base = stats[2 * row], logs = stats[2 * row + 1];
-  const float H = ent[row];
-  int64_t t = -1;
-  float gl = 0.f;
-  if (target && g_lp) {
-    t = target[row];
-    gl = t == ignore ? 0.f : (t >= 0 && t < C) ? g_lp[row] : NAN;
-  }
-  float pull = gl;
-  if (g_top)
-    for (int i = 0; i < k; ++i) pull += g_top[row * k + i];
-  const float gh = g_ent ? g_ent[row] : 0.f;
-  const bool none = logs == INFINITY;
-  for (int j = threadIdx.x; j < C; j += 256) {
-    float g = 0.f;
-    if (!none) {
-      const float l = ((float)zr[j] - base) - logs;
-      const float p = __expf(l);
-      g = -p * (pull + gh * (fmaxf(l, -1e30f) + H));
-      if (j == t) g += gl;
-      if (g_top)
-        for (int i = 0; i < k; ++i)
-          if (top_idx[row * k + i] == j) g += g_top[row * k + i];
+    const float* __restrict__ g_top, int64_t rows, int C, int k,
+    int tile_rows, int col_tiles, uint64_t magic, T* __restrict__ dz) {
+  __shared__ __align__(16) float tile[kTileElems];
+  __shared__ RowPull info[kTileRows];
+  constexpr int E = 16 / sizeof(T);
+  const int64_t row0 = blockIdx.x / col_tiles * (int64_t)tile_rows;
+  const int c0 = blockIdx.x % col_tiles * kTileElems;
+  const int many = (int)min((int64_t)tile_rows, rows - row0);
+  const int W = min(kTileElems, C - c0);  // = C where a tile has many rows
+  const int n = many * W;
+  if (threadIdx.x < many) {
+    const int64_t row = row0 + threadIdx.x;
+    RowPull p;
+    p.base = stats[2 * row];
+    p.logs = stats[2 * row + 1];
+    p.pull = 0.f;
+    if (target && g_lp) {
+      const int64_t t = target[row];
+      p.pull = t == ignore ? 0.f : (t >= 0 && t < C) ? g_lp[row] : NAN;
     }
-    out[j] = (T)g;
+    if (g_top)
+      for (int i = 0; i < k; ++i) p.pull += g_top[row * k + i];
+    p.gh = g_ent ? g_ent[row] : 0.f;
+    p.ent = ent[row];
+    info[threadIdx.x] = p;
+  }
+  __syncthreads();
+  const T* src = z + row0 * zs + c0;
+  const bool flat = zs == W || many == 1;
+  for (int i = threadIdx.x * E; i < n; i += 256 * E) {
+    // i / W by a product: exact for i below 2^12
+    int r = (int)((i * magic) >> 32), c = i - r * W;
+    union { Chunk q; T e[E]; } u;
+    if (flat && i + E <= n) {
+      u.q = *reinterpret_cast<const LooseChunk*>(src + i);
+    } else {
+      int rr = r, cc = c;
+#pragma unroll
+      for (int e = 0; e < E; ++e) {
+        if (i + e < n) u.e[e] = src[rr * zs + cc];
+        if (++cc == W) cc = 0, ++rr;
+      }
+    }
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+      if (i + e < n) {
+        const RowPull& p = info[r];
+        const float l = ((float)u.e[e] - p.base) - p.logs;
+        const float g =
+            -__expf(l) * (p.pull + p.gh * (fmaxf(l, -1e30f) + p.ent));
+        tile[i + e] = p.logs == INFINITY ? 0.f : g;
+      }
+      if (++c == W) c = 0, ++r;
+    }
+  }
+  __syncthreads();
+  if (g_top)
+    for (int i = threadIdx.x; i < many * k; i += 256) {
+      const int r = i / k;
+      const int64_t j = top_idx[row0 * k + i] - c0;
+      if (j >= 0 && j < W && info[r].logs != INFINITY)
+        tile[r * W + j] += g_top[row0 * k + i];
+    }
+  __syncthreads();
+  if (target && g_lp && threadIdx.x < many) {
+    const int64_t t = target[row0 + threadIdx.x];
+    if (t != ignore && t >= c0 && t < c0 + W && info[threadIdx.x].logs != INFINITY)
+      tile[threadIdx.x * W + (t - c0)] += g_lp[row0 + threadIdx.x];
+  }
+  __syncthreads();
+  T* out = dz + row0 * C + c0;  // rows of a tile follow each other
+  for (int i = threadIdx.x * E; i < n; i += 256 * E) {
+    union { Chunk q; T e[E]; } u;
+#pragma unroll
+    for (int e = 0; e < E; ++e)
+      u.e[e] = i + e < n ? (T)tile[i + e] : (T)0.f;
+    if (i + E <= n) {
+      *reinterpret_cast<LooseChunk*>(out + i) = u.q;
+    } else {
+#pragma unroll
+      for (int e = 0; e < E; ++e)
+        if (i + e < n) out[i + e] = u.e[e];
+    }
   }
 }
 
@@ -167,17 +619,73 @@ log_probs_fwd(at::Tensor logits, c10::optional<at::Tensor> target, int64_t k,
   auto top_lp = at::empty({rows, k}, f32);
   auto top_idx = at::empty({rows, k}, logits.options().dtype(at::kLong));
   auto stats = at::empty({rows, 2}, f32);
-  if (rows > 0)
-    DOA_FLOAT_TYPES(logits.scalar_type(), "log_probs", [&] {
-      TORCH_CHECK(rows < INT32_MAX, "log_probs: too many rows");
-      hipLaunchKernelGGL(
-          (log_probs_kernel<T>), dim3(rows), dim3(256), 0, stream_of_current(),
-          (const T*)zc.data_ptr(), zc.stride(0),
-          target.has_value() ? target->data_ptr<int64_t>() : nullptr, ignore,
-          (int)C, (int)k, lp.defined() ? lp.data_ptr<float>() : nullptr,
-          ent.data_ptr<float>(), top_lp.data_ptr<float>(),
-          top_idx.data_ptr<int64_t>(), stats.data_ptr<float>());
-    });
+  if (rows == 0) return {lp, ent, top_lp, top_idx, stats};
+  const int64_t* tp = target.has_value() ? target->data_ptr<int64_t>() : nullptr;
+  float* lpp = lp.defined() ? lp.data_ptr<float>() : nullptr;
+  auto stream = stream_of_current();
+  DOA_FLOAT_TYPES(logits.scalar_type(), "log_probs", [&] {
+    const T* zp = (const T*)zc.data_ptr();
+    const int64_t zs = zc.stride(0);
+    const int64_t row_bytes = C * sizeof(T);
+    if (row_bytes <= 2048) {
+      // lanes a row: as many as keep a wave's rows at 8 KiB of LDS, more where
+      // there are too few rows for 1024 waves
+      int L = row_bytes <= 128 ? 1 : row_bytes <= 512 ? 4 : 16;
+      while (L < 16 && rows * L < 64 * 1024) L *= 4;
+      const int wave_bytes = (int)ceil_div(64 / L * row_bytes, 16) * 16;
+      const int64_t blocks = ceil_div(rows, 4 * (64 / L));
+      TORCH_CHECK(blocks < INT32_MAX, "log_probs: too many rows");
+      auto go = [&](auto lv, auto kv) {
+        hipLaunchKernelGGL(
+            (log_probs_short_kernel<T, decltype(lv)::value,
+                                    decltype(kv)::value>),
+            dim3(blocks), dim3(256), 4 * wave_bytes, stream, zp, zs, tp, ignore,
+            rows, (int)C, (int)k, lpp, ent.data_ptr<float>(),
+            top_lp.data_ptr<float>(), top_idx.data_ptr<int64_t>(),
+            stats.data_ptr<float>(), wave_bytes);
+      };
+      auto slots = [&](auto lv) {  // registers for the next such number of keys
+        if (k == 0) go(lv, std::integral_constant<int, 0>{});
+        else if (k == 1) go(lv, std::integral_constant<int, 1>{});
+        else if (k <= 5) go(lv, std::integral_constant<int, 5>{});
+        else if (k <= 10) go(lv, std::integral_constant<int, 10>{});
+        else go(lv, std::integral_constant<int, kTopMost>{});
+      };
+      if (L == 1) slots(std::integral_constant<int, 1>{});
+      else if (L == 4) slots(std::integral_constant<int, 4>{});
+      else slots(std::integral_constant<int, 16>{});
+      return;
+    }
+    auto go = [&](auto nv) {
+      constexpr int NT = decltype(nv)::value, most = NT * kPer;
+      const int64_t splits = ceil_div(C, most);
+      const int chunk = (int)ceil_div(ceil_div(C, splits), 16) * 16;
+      TORCH_CHECK(rows * splits < INT32_MAX, "log_probs: too many rows");
+      at::Tensor sums, keys;
+      if (splits > 1) {
+        sums = at::empty({rows * splits * 3}, f32);
+        keys = at::empty({rows * splits * k}, top_idx.options());
+      }
+      float* sp = splits > 1 ? sums.data_ptr<float>() : nullptr;
+      uint64_t* kp =
+          splits > 1 ? (uint64_t*)keys.data_ptr<int64_t>() : nullptr;
+      hipLaunchKernelGGL((log_probs_long_kernel<T, NT>), dim3(rows * splits),
+                         dim3(NT), 0, stream, zp, zs, tp, ignore, (int)C,
+                         (int)k, (int)splits, chunk, lpp,
+                         ent.data_ptr<float>(), top_lp.data_ptr<float>(),
+                         top_idx.data_ptr<int64_t>(), stats.data_ptr<float>(),
+                         sp, kp);
+      if (splits > 1)
+        hipLaunchKernelGGL((log_probs_join_kernel<T>), dim3(rows), dim3(256), 0,
+                           stream, zp, zs, tp, ignore, (int)C, (int)k,
+                           (int)splits, sp, kp, lpp, ent.data_ptr<float>(),
+                           top_lp.data_ptr<float>(),
+                           top_idx.data_ptr<int64_t>(),
+                           stats.data_ptr<float>());
+    };
+    if (C <= 256 * kPer) go(std::integral_constant<int, 256>{});
+    else go(std::integral_constant<int, 1024>{});
+  });
   DOA_CHECK_HIP(hipGetLastError());
   return {lp, ent, top_lp, top_idx, stats};
 }
@@ -202,16 +710,24 @@ at::Tensor log_probs_bwd(at::Tensor logits, c10::optional<at::Tensor> target,
                   "log_probs: gradient of another shape or type");
       gp[i] = keep[i].data_ptr<float>();
     }
-  if (rows > 0)
-    DOA_FLOAT_TYPES(logits.scalar_type(), "log_probs", [&] {
-      hipLaunchKernelGGL(
-          (log_probs_bwd_kernel<T>), dim3(rows), dim3(256), 0,
-          stream_of_current(), (const T*)zc.data_ptr(), zc.stride(0),
-          target.has_value() ? target->data_ptr<int64_t>() : nullptr, ignore,
-          top_idx.data_ptr<int64_t>(), stats.data_ptr<float>(),
-          ent.data_ptr<float>(), gp[0], gp[1], gp[2], (int)C, (int)k,
-          (T*)dz.data_ptr());
-    });
+  if (rows == 0) return dz;
+  const int64_t W = std::min<int64_t>(C, kTileElems);
+  const int64_t col_tiles = ceil_div(C, kTileElems);
+  // rows a tile: what fits, but at least 1024 tiles where there are the rows
+  const int64_t tile_rows = std::max<int64_t>(
+      1, std::min<int64_t>({kTileRows, kTileElems / W, ceil_div(rows, 1024)}));
+  const int64_t blocks = ceil_div(rows, tile_rows) * col_tiles;
+  TORCH_CHECK(blocks < INT32_MAX, "log_probs: too many rows");
+  const uint64_t magic = ((uint64_t)1 << 32) / W + 1;
+  DOA_FLOAT_TYPES(logits.scalar_type(), "log_probs", [&] {
+    hipLaunchKernelGGL(
+        (log_probs_bwd_kernel<T>), dim3(blocks), dim3(256), 0,
+        stream_of_current(), (const T*)zc.data_ptr(), zc.stride(0),
+        target.has_value() ? target->data_ptr<int64_t>() : nullptr, ignore,
+        top_idx.data_ptr<int64_t>(), stats.data_ptr<float>(),
+        ent.data_ptr<float>(), gp[0], gp[1], gp[2], rows, (int)C, (int)k,
+        (int)tile_rows, (int)col_tiles, magic, (T*)dz.data_ptr());
+  });
   DOA_CHECK_HIP(hipGetLastError());
   return dz;
 }

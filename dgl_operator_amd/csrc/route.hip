@@ -78,7 +78,7 @@ __device__ inline void place_tile(const IdT* ids, int64_t lo, int64_t hi,
       if ((same >> lane) == 1ull) next[id] = p + 1;
       source[p] = (int)f;
     }
-    __builtin_amdgcn_wave_barrier();
+    wave_sync();
     if (f < hi) position[f] = p;
   }
 }
@@ -95,7 +95,7 @@ __global__ __launch_bounds__(1024) void route_small_kernel(
   const int waves = blockDim.x >> 6;
   int* mine = hist + wave * G;
   for (int g = lane; g < G; g += 64) mine[g] = 0;
-  __builtin_amdgcn_wave_barrier();
+  wave_sync();
   const int lo = wave * tile, hi = min(n, lo + tile);
   for (int f = lo + lane; f < hi; f += 64) {
     const int id = load_id(ids, f, n, G);
@@ -136,14 +136,14 @@ __global__ __launch_bounds__(256) void route_count_kernel(
   const int t = blockIdx.x * (blockDim.x >> 6) + wave;
   int* mine = hist + wave * G;
   for (int g = lane; g < G; g += 64) mine[g] = 0;
-  __builtin_amdgcn_wave_barrier();
+  wave_sync();
   if (t >= tiles) return;
   const int64_t lo = (int64_t)t * tile, hi = min(n, lo + tile);
   for (int64_t f = lo + lane; f < hi; f += 64) {
     const int id = load_id(ids, f, n, G);
     if (id >= 0) atomicAdd(&mine[id], 1);
   }
-  __builtin_amdgcn_wave_barrier();
+  wave_sync();
   for (int g = lane; g < G; g += 64) counts[(int64_t)g * tiles + t] = mine[g];
 }
 

@@ -31,9 +31,6 @@ using f32x4 = __attribute__((__vector_size__(4 * sizeof(float)))) float;
 
 constexpr int kStepBytes = 128;
 
-using Chunk = uint32_t __attribute__((ext_vector_type(4)));
-typedef Chunk LooseChunk __attribute__((aligned(2)));  // at any element
-
 template <typename T, bool COL, int CHUNKS>
 __device__ inline int swizzle(int chunk, int outer) {
   if constexpr (!COL) return chunk ^ ((outer ^ (outer >> 3)) & 7);
@@ -363,10 +360,10 @@ __global__ __launch_bounds__(256) void sum_parts_kernel(
     if (i + 4 <= n) {
       float s[4] = {};
       for (int p = 0; p < splits; ++p) {
-        const auto v =
-            *reinterpret_cast<const LooseVec<float, 4>*>(parts + p * n + i);
+        union { Chunk q; float v[4]; } u;
+        u.q = *reinterpret_cast<const LooseChunk*>(parts + p * n + i);
 #pragma unroll
-        for (int e = 0; e < 4; ++e) s[e] += v.v[e];
+        for (int e = 0; e < 4; ++e) s[e] += u.v[e];
       }
 #pragma unroll
       for (int e = 0; e < 4; ++e) out[i + e] = (T)s[e];

@@ -14,20 +14,15 @@ struct alignas(sizeof(T) * V) Vec {
   T v[V];
 };
 
-// the same with no alignment beyond an element's: rows of odd length start
-// anywhere, and gfx950 loads 16 bytes from any element's address
-template <typename T, int V>
-struct __attribute__((packed, aligned(sizeof(T)))) LooseVec {
-  T v[V];
-};
+// what the wave's lanes wrote to LDS is there for its other lanes
+__device__ inline void wave_sync() {
+  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+  __builtin_amdgcn_wave_barrier();
+}
 
-// device types of the tensors' types (hardware conversions, unlike c10's)
-template <typename T>
-struct DeviceT { using type = T; };
-template <>
-struct DeviceT<c10::Half> { using type = _Float16; };
-template <>
-struct DeviceT<c10::BFloat16> { using type = __bf16; };
+// 16 bytes, also at any 2-byte address: gfx950 loads them all the same
+using Chunk = uint32_t __attribute__((ext_vector_type(4)));
+typedef Chunk LooseChunk __attribute__((aligned(2)));
 
 inline hipStream_t stream_of_current() {
   return c10::hip::getCurrentHIPStream().stream();

@@ -60,24 +60,15 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor> cpdist_neg_bwd(
 
 std::tuple<at::Tensor, at::Tensor, at::Tensor> route_rows(at::Tensor ids,
                                                           int64_t groups);
-at::Tensor dispatch_rows(at::Tensor x, at::Tensor position,
-                         at::Tensor offsets);
-at::Tensor combine_rows(at::Tensor y, at::Tensor position,
-                        c10::optional<at::Tensor> weights);
-std::tuple<at::Tensor, at::Tensor> combine_rows_bwd(
-    at::Tensor gout, c10::optional<at::Tensor> y, at::Tensor position,
-    at::Tensor offsets, c10::optional<at::Tensor> weights, bool want_y);
-at::Tensor segment_mm(at::Tensor offsets, at::Tensor x, at::Tensor weight,
-                      bool transposed);
 at::Tensor segment_mm_wgrad(at::Tensor offsets, at::Tensor x, at::Tensor grad);
-std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor, at::Tensor>
-log_probs_fwd(at::Tensor logits, c10::optional<at::Tensor> target, int64_t k,
-              int64_t ignore);
-at::Tensor log_probs_bwd(at::Tensor logits, c10::optional<at::Tensor> target,
-                         int64_t ignore, at::Tensor top_idx, at::Tensor stats,
-                         at::Tensor ent, c10::optional<at::Tensor> g_lp,
-                         c10::optional<at::Tensor> g_ent,
-                         c10::optional<at::Tensor> g_top);
+at::Tensor dispatch_rows_ad(at::Tensor x, at::Tensor position,
+                            at::Tensor offsets);
+at::Tensor combine_rows_ad(at::Tensor y, c10::optional<at::Tensor> weights,
+                           at::Tensor position, at::Tensor offsets);
+at::Tensor segment_mm_ad(at::Tensor offsets, at::Tensor x, at::Tensor weight);
+std::vector<at::Tensor> log_probs_ad(at::Tensor logits,
+                                     c10::optional<at::Tensor> target,
+                                     int64_t k, int64_t ignore);
 
 }  // namespace doa
 
@@ -117,11 +108,9 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("cpdist_neg_fwd", &doa::cpdist_neg_fwd);
   m.def("cpdist_neg_bwd", &doa::cpdist_neg_bwd);
   m.def("route_rows", &doa::route_rows);
-  m.def("dispatch_rows", &doa::dispatch_rows);
-  m.def("combine_rows", &doa::combine_rows);
-  m.def("combine_rows_bwd", &doa::combine_rows_bwd);
-  m.def("segment_mm", &doa::segment_mm);
+  m.def("dispatch_rows", &doa::dispatch_rows_ad);
+  m.def("combine_rows", &doa::combine_rows_ad);
+  m.def("segment_mm", &doa::segment_mm_ad);
   m.def("segment_mm_wgrad", &doa::segment_mm_wgrad);
-  m.def("log_probs_fwd", &doa::log_probs_fwd);
-  m.def("log_probs_bwd", &doa::log_probs_bwd);
+  m.def("log_probs", &doa::log_probs_ad);
 }

@@ -28,6 +28,7 @@ SOURCES = [
     "route.hip",
     "segment_mm.hip",
     "log_probs.hip",
+    "autograd.cpp",
     "ldg.cpp",
     "bindings.cpp",
 ]

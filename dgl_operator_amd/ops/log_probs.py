@@ -76,33 +76,24 @@ def _bwd_ref(logits, target, ignore_index, logp, none, entropy, index,
 
 
 class _LogProbs(torch.autograd.Function):
+    """CPU path; the GPU's is csrc/autograd.cpp."""
+
     @staticmethod
     def forward(ctx, logits, target, top_k, ignore_index):
         ctx.set_materialize_grads(False)
         ctx.ignore_index = ignore_index
-        if logits.is_cuda:
-            ext = backend.ext_for(logits)
-            lp, ent, top, index, stats = ext.log_probs_fwd(
-                logits, target, top_k, ignore_index)
-            ctx.save_for_backward(logits, target, index, stats, ent)
-        else:
-            lp, ent, top, index, logp, none = _fwd_ref(
-                logits, target, top_k, ignore_index)
-            ctx.save_for_backward(logits, target, index, logp, ent, none)
+        lp, ent, top, index, logp, none = _fwd_ref(
+            logits, target, top_k, ignore_index)
+        ctx.save_for_backward(logits, target, index, logp, ent, none)
         ctx.mark_non_differentiable(index)
         return lp, ent, top, index
 
     @staticmethod
     @once_differentiable
     def backward(ctx, g_lp, g_ent, g_top, _):
-        logits, target, index, saved, ent, *none = ctx.saved_tensors
-        if logits.is_cuda:
-            ext = backend.ext_for(logits)
-            dz = ext.log_probs_bwd(logits, target, ctx.ignore_index, index,
-                                   saved, ent, g_lp, g_ent, g_top)
-        else:
-            dz = _bwd_ref(logits, target, ctx.ignore_index, saved, none[0],
-                          ent, index, g_lp, g_ent, g_top)
+        logits, target, index, logp, ent, none = ctx.saved_tensors
+        dz = _bwd_ref(logits, target, ctx.ignore_index, logp, none, ent, index,
+                      g_lp, g_ent, g_top)
         return dz, None, None, None
 
 
@@ -139,12 +130,17 @@ def log_probs(
             "log_probs: target and logits are on different devices"
         assert not target.is_floating_point() and target.dtype != torch.bool, \
             "log_probs: integer targets expected"
-        target = target.reshape(-1).long()
+        target = target.reshape(-1).long().contiguous()
     rows = 1
     for d in lead:
         rows *= d
-    lp, ent, top, index = _LogProbs.apply(
-        logits.reshape(rows, C), target, top_k, ignore_index)
+    flat = logits if logits.dim() == 2 else logits.reshape(rows, C)
+    if logits.is_cuda:
+        ext = backend.ext_for(logits)
+        ent, top, index, *lp = ext.log_probs(flat, target, top_k, ignore_index)
+        lp = lp[0] if lp else None
+    else:
+        lp, ent, top, index = _LogProbs.apply(flat, target, top_k, ignore_index)
     if len(lead) != 1:
         lp = lp.view(lead) if lp is not None else None
         ent = ent.view(lead)

@@ -93,66 +93,48 @@ def _combine_ref(y, position, weights):
 
 
 class _DispatchRows(torch.autograd.Function):
+    """CPU path; the GPU's is csrc/autograd.cpp."""
+
     @staticmethod
-    def forward(ctx, x, position, offsets):
+    def forward(ctx, x, position):
         ctx.save_for_backward(position)
-        if x.is_cuda:
-            ext = backend.ext_for(x)
-            return ext.dispatch_rows(x, position, offsets)
         return _dispatch_ref(x, position)
 
     @staticmethod
     @once_differentiable
     def backward(ctx, grad_out):
         (position,) = ctx.saved_tensors
-        if grad_out.is_cuda:
-            ext = backend.ext_for(grad_out)
-            return ext.combine_rows(grad_out, position, None), None, None
-        return _combine_ref(grad_out, position, None), None, None
+        return _combine_ref(grad_out, position, None), None
 
 
 class _CombineRows(torch.autograd.Function):
+    """CPU path; the GPU's is csrc/autograd.cpp."""
+
     @staticmethod
-    def forward(ctx, y, weights, position, offsets):
-        # the weights act in 32 bits whatever they come in
-        w = weights
-        if w is not None and y.is_cuda:
-            w = w.float().contiguous()
-        want_w = weights is not None and ctx.needs_input_grad[1]
-        ctx.save_for_backward(y if want_w else None, w, position, offsets)
-        ctx.weight_dtype = weights.dtype if weights is not None else None
-        if y.is_cuda:
-            ext = backend.ext_for(y)
-            return ext.combine_rows(y, position, w)
+    def forward(ctx, y, weights, position):
+        ctx.save_for_backward(y, weights, position)
         return _combine_ref(y, position, weights)
 
     @staticmethod
     @once_differentiable
     def backward(ctx, grad_out):
-        y, w, position, offsets = ctx.saved_tensors
-        want_y, want_w = ctx.needs_input_grad[:2]
-        if grad_out.is_cuda:
-            ext = backend.ext_for(grad_out)
-            dy, dw = ext.combine_rows_bwd(
-                grad_out, y if want_w else None, position, offsets, w, want_y)
-        else:
-            dy = dw = None
-            rows, k = position.shape
-            if want_y:
-                g = grad_out.unsqueeze(1).expand(rows, k, grad_out.shape[1])
-                if w is not None:
-                    g = (g.to(torch.promote_types(g.dtype, torch.float32))
-                         * w.unsqueeze(-1)).to(grad_out.dtype)
-                flat = position.reshape(-1).long()
-                kept = (flat >= 0).nonzero()[:, 0]
-                dy = grad_out.new_zeros((rows * k, grad_out.shape[1]))
-                dy[flat[kept]] = g.reshape(rows * k, -1)[kept]
-            if want_w:
-                taken = _taken_ref(y, position)
-                dw = (taken * grad_out.to(taken.dtype).unsqueeze(1)).sum(-1)
-        if dw is not None:
-            dw = dw.to(ctx.weight_dtype)
-        return dy, dw, None, None
+        y, w, position = ctx.saved_tensors
+        dy = dw = None
+        rows, k = position.shape
+        if ctx.needs_input_grad[0]:
+            g = grad_out.unsqueeze(1).expand(rows, k, grad_out.shape[1])
+            if w is not None:
+                g = (g.to(torch.promote_types(g.dtype, torch.float32))
+                     * w.unsqueeze(-1)).to(grad_out.dtype)
+            flat = position.reshape(-1).long()
+            kept = (flat >= 0).nonzero()[:, 0]
+            dy = grad_out.new_zeros((rows * k, grad_out.shape[1]))
+            dy[flat[kept]] = g.reshape(rows * k, -1)[kept]
+        if ctx.needs_input_grad[1]:
+            taken = _taken_ref(y, position)
+            dw = (taken * grad_out.to(taken.dtype).unsqueeze(1)).sum(-1)
+            dw = dw.to(w.dtype)
+        return dy, dw, None
 
 
 def dispatch_rows(route: RowRoute, x: torch.Tensor) -> torch.Tensor:
@@ -165,7 +147,13 @@ def dispatch_rows(route: RowRoute, x: torch.Tensor) -> torch.Tensor:
     assert x.device == route.position.device, \
         "dispatch_rows: rows and plan are on different devices"
     assert x.is_floating_point(), "dispatch_rows: floating point rows expected"
-    out = _DispatchRows.apply(_flat(x), route.position, route.offsets)
+    if x.is_cuda:
+        ext = backend.ext_for(x)
+        out = ext.dispatch_rows(_flat(x), route.position, route.offsets)
+    else:
+        out = _DispatchRows.apply(_flat(x), route.position)
+    if x.dim() == 2:
+        return out
     return out.view((rows * k,) + x.shape[1:])
 
 
@@ -190,7 +178,13 @@ def combine_rows(
             f"combine_rows: weights must be [{rows}, {k}]"
         assert weights.device == y.device and weights.is_floating_point(), \
             "combine_rows: floating point weights on the rows' device expected"
-    out = _CombineRows.apply(_flat(y), weights, route.position, route.offsets)
+    if y.is_cuda:
+        ext = backend.ext_for(y)
+        out = ext.combine_rows(_flat(y), weights, route.position, route.offsets)
+    else:
+        out = _CombineRows.apply(_flat(y), weights, route.position)
+    if y.dim() == 2:
+        return out
     return out.view((rows,) + y.shape[1:])
 
 

@@ -32,37 +32,25 @@ def _segment_mm_ref(offsets, x, weight):
 
 
 class _SegmentMM(torch.autograd.Function):
+    """CPU path; the GPU's is csrc/autograd.cpp."""
+
     @staticmethod
     def forward(ctx, offsets, x, weight):
-        need_x, need_w = ctx.needs_input_grad[1:]
-        ctx.save_for_backward(offsets, x if need_w else None,
-                              weight if need_x else None)
-        if x.is_cuda:
-            ext = backend.ext_for(x)
-            return ext.segment_mm(offsets, x, weight, False)
+        ctx.save_for_backward(offsets, x, weight)
         return _segment_mm_ref(offsets, x, weight)
 
     @staticmethod
     @once_differentiable
     def backward(ctx, grad_out):
         offsets, x, weight = ctx.saved_tensors
-        need_x, need_w = ctx.needs_input_grad[1:]
         dx = dw = None
-        if grad_out.is_cuda:
-            ext = backend.ext_for(grad_out)
-            if need_x:
-                dx = ext.segment_mm(offsets, grad_out, weight, True)
-            if need_w:
-                dw = ext.segment_mm_wgrad(offsets, x, grad_out)
-        else:
-            if need_x:
-                dx = _segment_mm_ref(offsets, grad_out, weight.transpose(1, 2))
-            if need_w:
-                dw = x.new_zeros((offsets.numel() - 1, x.shape[1],
-                                  grad_out.shape[1]))
-                for g, a, b in _bounds(offsets, x.shape[0]):
-                    dw[g] = (_wide(x[a:b]).t() @ _wide(grad_out[a:b])
-                             ).to(dw.dtype)
+        if ctx.needs_input_grad[1]:
+            dx = _segment_mm_ref(offsets, grad_out, weight.transpose(1, 2))
+        if ctx.needs_input_grad[2]:
+            dw = x.new_zeros((offsets.numel() - 1, x.shape[1],
+                              grad_out.shape[1]))
+            for g, a, b in _bounds(offsets, x.shape[0]):
+                dw[g] = (_wide(x[a:b]).t() @ _wide(grad_out[a:b])).to(dw.dtype)
         return None, dx, dw
 
 
@@ -90,4 +78,7 @@ def segment_mm(offsets: torch.Tensor, x: torch.Tensor,
         "segment_mm: x and weight must share a floating point type"
     assert x.device == weight.device == offsets.device, \
         "segment_mm: all tensors must be on one device"
-    return _SegmentMM.apply(offsets.contiguous(), x, weight)
+    offsets = offsets.contiguous()
+    if x.is_cuda:
+        return backend.ext_for(x).segment_mm(offsets, x, weight)
+    return _SegmentMM.apply(offsets, x, weight)

@@ -369,6 +369,30 @@ def test_log_probs_partial_gradients(dev):
         assert (g.cpu().double() - h).abs().max() < 64 * 10 * 4 * oracle.U
 
 
+def test_log_probs_strided_targets(dev):
+    z = torch.randn(5, 3, 7, device=dev)
+    t = torch.randint(0, 7, (3, 5), device=dev)
+    a = ops.log_probs(z, t.t())
+    b = ops.log_probs(z.reshape(15, 7), t.t().reshape(15).int())
+    assert torch.equal(a.log_prob.reshape(15), b.log_prob)
+    c = ops.log_probs(z[:, 0], t[0].repeat_interleave(2)[::2])
+    assert torch.equal(c.log_prob, a.log_prob[:, 0])
+
+
+def test_second_derivatives_are_refused(dev):
+    """A first derivative may be part of a graph; a second one raises."""
+    x = torch.randn(4, 6, device=dev, requires_grad=True)
+    w = torch.randn(2, 6, 6, device=dev, requires_grad=True)
+    p = torch.rand(4, 1, device=dev, requires_grad=True)
+    route = ops.route_rows(torch.tensor([0, 1, 1, 0], device=dev), 2)
+    for y in (ops.dispatch_rows(route, x), ops.combine_rows(route, x, p),
+              ops.segment_mm(route.offsets, x, w),
+              ops.log_probs(x).entropy):
+        g, = torch.autograd.grad((y * y).sum(), x, create_graph=True)
+        with pytest.raises(RuntimeError, match="differentiate twice"):
+            g.sum().backward()
+
+
 def test_log_probs_refuses(dev):
     z = torch.zeros(3, 40, device=dev)
     with pytest.raises(RuntimeError, match="top_k"):

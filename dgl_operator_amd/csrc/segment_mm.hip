@@ -26,14 +26,17 @@ using f32x4 = __attribute__((__vector_size__(4 * sizeof(float)))) float;
 // depths (l >> 4) * 8 .. + 8, what the matrix instruction wants.
 //
 // 16-byte chunks are swizzled so that neither read meets a bank twice: row
-// tiles by key(r) = (r ^ r >> 3) & 7 over the row's 8 chunks, col tiles by the
-// depth over 32 bytes (halves, two depth quads a read) or 64 (floats).
+// tiles by (r >> 1) & 7 over a row's 8 chunks, or -(r >> 2) & 3 over 4 (16 lanes
+// of a 16-byte read meet in rows 0-3, 12-15 of one depth and 4-11 of the next),
+// col tiles by the depth over 32 bytes (halves, two depth quads a read) or 64
+// (floats).
 
 constexpr int kStepBytes = 128;
 
 template <typename T, bool COL, int CHUNKS>
 __device__ inline int swizzle(int chunk, int outer) {
-  if constexpr (!COL) return chunk ^ ((outer ^ (outer >> 3)) & 7);
+  if constexpr (!COL && CHUNKS == 4) return chunk ^ (-(outer >> 2) & 3);
+  if constexpr (!COL) return chunk ^ ((outer >> 1) & 7);
   if constexpr (sizeof(T) == 2 && CHUNKS >= 16)
     return chunk ^ (((outer & 3) | ((outer >> 1) & 4)) << 1);
   if constexpr (sizeof(T) == 2)
@@ -41,13 +44,21 @@ __device__ inline int swizzle(int chunk, int outer) {
   return chunk ^ (((outer >> 2) & 3) << 2);
 }
 
+// the thread's index, in a way that what depends on it is computed where it is
+// used: kept across a loop it would cost the accumulators their registers
+__device__ inline int thread_here() {
+  int t = threadIdx.x;
+  asm volatile("" : "+v"(t));
+  return t;
+}
+
 // one operand's tile: SIDE rows (or columns) by BK of depth
-template <typename T, bool COL, int SIDE, int THREADS>
+template <typename T, bool COL, int SIDE, int THREADS, int STEP = kStepBytes>
 struct Tile {
   static constexpr int E = 16 / sizeof(T);                  // a chunk
-  static constexpr int BK = kStepBytes / sizeof(T);
+  static constexpr int BK = STEP / sizeof(T);
   static constexpr int CHUNKS = COL ? SIDE / E : BK / E;    // an outer index
-  static constexpr int BYTES = SIDE * kStepBytes;
+  static constexpr int BYTES = SIDE * STEP;
   static constexpr int PER = BYTES / 16 / THREADS;          // chunks a thread
   static_assert(PER * THREADS * 16 == BYTES, "tile and threads do not match");
   static_assert(!COL || CHUNKS >= (sizeof(T) == 2 ? 8 : 16), "swizzle");
@@ -56,9 +67,10 @@ struct Tile {
   // those beyond the `side` rows there are.
   static constexpr uint32_t kOut = 0x80000000u;
   static __device__ void place(int64_t ld, int side, uint32_t* at) {
+    const int thread = thread_here();
 #pragma unroll
     for (int i = 0; i < PER; ++i) {
-      const int id = i * THREADS + threadIdx.x, o = id / CHUNKS;
+      const int id = i * THREADS + thread, o = id / CHUNKS;
       const int c = swizzle<T, COL, CHUNKS>(id % CHUNKS, o) * E;
       at[i] = (COL ? c : o) < side ? (uint32_t)((o * ld + c) * sizeof(T)) : kOut;
     }
@@ -78,14 +90,7 @@ struct Tile {
     const uint32_t to = __builtin_amdgcn_readfirstlane(
         (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char*)lds +
         (threadIdx.x >> 6) * 1024);
-#pragma unroll
-    for (int i = 0; i < PER; ++i) {
-      uint32_t v = at[i];
-      if (depth < BK) {
-        const int id = i * THREADS + threadIdx.x, o = id / CHUNKS;
-        const int k = COL ? o : swizzle<T, COL, CHUNKS>(id % CHUNKS, o) * E;
-        if (k >= depth) v = kOut;
-      }
+    auto issue = [&](int i, uint32_t v) {
       asm volatile(
           "s_mov_b32 m0, %0\n\t"
           "s_nop 0\n\t"
@@ -93,6 +98,18 @@ struct Tile {
           :
           : "s"(to + i * THREADS * 16), "v"(v), "s"(rsrc)
           : "memory", "m0");
+    };
+    if (depth >= BK) {
+#pragma unroll
+      for (int i = 0; i < PER; ++i) issue(i, at[i]);
+    } else {
+      const int thread = thread_here();
+#pragma unroll
+      for (int i = 0; i < PER; ++i) {
+        const int id = i * THREADS + thread, o = id / CHUNKS;
+        const int k = COL ? o : swizzle<T, COL, CHUNKS>(id % CHUNKS, o) * E;
+        issue(i, k < depth ? at[i] : kOut);
+      }
     }
   }
   // the same through registers, element by element where a chunk is cut
@@ -123,39 +140,52 @@ struct Tile {
       *reinterpret_cast<Chunk*>(lds + (i * THREADS + threadIdx.x) * 16) = from[i];
   }
 
-  // the 16 x (4 E) fragment of rows s0.. at depth chunk step kk (0, 1)
+  // A wave's F fragments: 16 rows each from row s0 on, 4 E of depth at step kk.
+  // A row tile's swizzle is the same 16 rows further on, a col tile's is not.
   using Frag = __attribute__((__vector_size__(16))) T;
-  static __device__ Frag frag(const char* lds, int s0, int kk) {
-    const int lane = threadIdx.x & 63, q = lane >> 4, s = lane & 15;
-    if constexpr (!COL) {
-      const int r = s0 + s;
-      return *reinterpret_cast<const Frag*>(
-          lds + r * kStepBytes + swizzle<T, false, CHUNKS>(kk * 4 + q, r) * 16);
-    } else if constexpr (sizeof(T) == 2) {
-      using S4 = short __attribute__((ext_vector_type(4)));
-      const int col = s0 + (s & 3) * 4;
-      union { S4 h[2]; Frag f; } u;
+  template <int F>
+  struct Reader {
+    int at[COL ? F : 1];
+    __device__ explicit Reader(int s0) {
+      const int lane = threadIdx.x & 63, q = lane >> 4, s = lane & 15;
+      if constexpr (!COL) {
+        at[0] = (s0 + s) * STEP + swizzle<T, false, CHUNKS>(q, s0 + s) * 16;
+      } else {
+        // halves: 4 columns at depth q * 8 + (s >> 2); floats: column s at q * 4
+        const int k = sizeof(T) == 2 ? q * 8 + (s >> 2) : q * 4;
+        const int off = sizeof(T) == 2 ? (s & 3) * 4 : s;
 #pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        const int k = kk * 32 + q * 8 + h * 4 + (s >> 2);
-        const char* a = lds + k * (SIDE * 2) +
-                        swizzle<T, true, CHUNKS>(col / 8, k) * 16 + (col & 4) * 2;
-        u.h[h] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-            (__attribute__((address_space(3))) S4*)a);
+        for (int f = 0; f < F; ++f) {
+          const int col = s0 + f * 16 + off;
+          at[f] = k * (SIDE * (int)sizeof(T)) +
+                  swizzle<T, true, CHUNKS>(col / E, k) * 16 +
+                  col % E * (int)sizeof(T);
+        }
       }
-      return u.f;
-    } else {
-      Frag f;
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int k = kk * 16 + q * 4 + i, col = s0 + s;
-        f[i] = *reinterpret_cast<const T*>(
-            lds + k * (SIDE * 4) + swizzle<T, true, CHUNKS>(col / 4, k) * 16 +
-            (col & 3) * 4);
-      }
-      return f;
     }
-  }
+    __device__ Frag get(const char* lds, int f, int kk) const {
+      if constexpr (!COL) {
+        return *reinterpret_cast<const Frag*>(
+            lds + (at[0] ^ (kk * 64)) + f * 16 * STEP);
+      } else if constexpr (sizeof(T) == 2) {
+        using S4 = short __attribute__((ext_vector_type(4)));
+        union { S4 h[2]; Frag f; } u;
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+          u.h[h] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+              (__attribute__((address_space(3))) S4*)(
+                  lds + at[f] + (kk * 32 + h * 4) * (SIDE * 2)));
+        return u.f;
+      } else {
+        Frag r;
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          r[i] = *reinterpret_cast<const T*>(
+              lds + at[f] + (kk * 16 + i) * (SIDE * 4));
+        return r;
+      }
+    }
+  };
 };
 
 template <typename T, typename Frag>
@@ -172,13 +202,53 @@ __device__ inline f32x4 mma(Frag a, Frag b, f32x4 c) {
   }
 }
 
-// four neighbours at once, at any element unless ALIGNED
-template <bool ALIGNED, typename O>
-__device__ inline void store4(O* p, const Vec<O, 4>& v) {
-  using U = uint32_t __attribute__((ext_vector_type(sizeof(O))));
-  typedef U L __attribute__((aligned(sizeof(O))));
-  using P = std::conditional_t<ALIGNED, U, L>;
-  *reinterpret_cast<P*>(p) = __builtin_bit_cast(U, v);
+// A wave's 16 FM x 16 FN results: strips of 16 rows go through `room` (ROOM
+// bytes of LDS, the wave's own) and out in whole lines of its columns; a row is
+// padded by 16 bytes to keep the strip's writes off one bank.
+template <typename T, typename O, bool WHOLE, int FM, int FN, int ROOM>
+__device__ inline void store_tile(const f32x4 (&acc)[FM][FN], char* room, O* c,
+                                  int64_t ldc, int M, int N) {
+  constexpr int E = 16 / sizeof(O), ROW = FN * 16 * sizeof(O) + 16;
+  constexpr int CHUNKS = FN * 16 / E;
+  constexpr int FIT = ROOM / (16 * ROW), STRIPS = FIT < FM ? FIT : FM;
+  static_assert(STRIPS >= 1, "no room for a strip");
+#pragma unroll
+  for (int i0 = 0; i0 < FM; i0 += STRIPS) {
+    wave_sync();  // the last strips are out
+    __builtin_amdgcn_sched_barrier(0);
+    const int lane = thread_here() & 63;
+#pragma unroll
+    for (int i = i0; i < FM && i < i0 + STRIPS; ++i)
+#pragma unroll
+      for (int j = 0; j < FN; ++j) {
+        Vec<O, 4> o;
+#pragma unroll
+        for (int r = 0; r < 4; ++r) o.v[r] = (O)acc[i][j][r];
+        *reinterpret_cast<Vec<O, 4>*>(
+            room + ((i - i0) * 16 + (lane & 15)) * ROW +
+            (j * 16 + (lane >> 4) * 4) * sizeof(O)) = o;
+      }
+    wave_sync();
+#pragma unroll
+    for (int i = i0; i < FM && i < i0 + STRIPS; ++i)
+#pragma unroll
+      for (int at = lane; at < 16 * CHUNKS; at += 64) {
+        const int r = at / CHUNKS, n = at % CHUNKS * E, m = i * 16 + r;
+        if (m >= M || n >= N) continue;
+        union { Chunk q; O v[E]; } u;
+        u.q = *reinterpret_cast<const Chunk*>(
+            room + ((i - i0) * 16 + r) * ROW + at % CHUNKS * 16);
+        O* to = c + m * ldc + n;
+        if (n + E <= N) {
+          if constexpr (WHOLE) *reinterpret_cast<Chunk*>(to) = u.q;
+          else *reinterpret_cast<LooseChunk*>(to) = u.q;
+        } else {
+#pragma unroll
+          for (int e = 0; e < E; ++e)
+            if (n + e < N) to[e] = u.v[e];
+        }
+      }
+  }
 }
 
 // c[m][n] = sum_k a(m, k) b(k, n) for one tile of BM x BN. AC, BC: that
@@ -195,8 +265,10 @@ __device__ inline void tile_product(const T* a, int64_t lda, int M, const T* b,
   constexpr int FM = BM / WM / 16, FN = BN / WN / 16;
   constexpr int BK = TA::BK;
   __shared__ __align__(16) char lds[2][TA::BYTES + TB::BYTES];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int wm = wave / WN * (BM / WM), wn = wave % WN * (BN / WN);
+  const typename TA::template Reader<FM> read_a(wm);
+  const typename TB::template Reader<FN> read_b(wn);
   f32x4 acc[FM][FN] = {};
   const int64_t step_a = AC ? BK * lda : BK, step_b = BC ? BK * ldb : BK;
   auto multiply = [&](const char* la, const char* lb) {
@@ -205,9 +277,9 @@ __device__ inline void tile_product(const T* a, int64_t lda, int M, const T* b,
       typename TA::Frag fa[FM];
       typename TB::Frag fb[FN];
 #pragma unroll
-      for (int i = 0; i < FM; ++i) fa[i] = TA::frag(la, wm + i * 16, kk);
+      for (int i = 0; i < FM; ++i) fa[i] = read_a.get(la, i, kk);
 #pragma unroll
-      for (int j = 0; j < FN; ++j) fb[j] = TB::frag(lb, wn + j * 16, kk);
+      for (int j = 0; j < FN; ++j) fb[j] = read_b.get(lb, j, kk);
 #pragma unroll
       for (int i = 0; i < FM; ++i)
 #pragma unroll
@@ -260,33 +332,47 @@ __device__ inline void tile_product(const T* a, int64_t lda, int M, const T* b,
       }
     }
   }
-#pragma unroll
-  for (int i = 0; i < FM; ++i) {
-    const int m = wm + i * 16 + (lane & 15);
-#pragma unroll
-    for (int j = 0; j < FN; ++j) {
-      const int n = wn + j * 16 + (lane >> 4) * 4;
-      if (m >= M) continue;
-      Vec<O, 4> o;
-#pragma unroll
-      for (int r = 0; r < 4; ++r) o.v[r] = (O)acc[i][j][r];
-      if constexpr (WHOLE) {
-        if (n < N) store4<true>(c + m * ldc + n, o);
-      } else if (n + 4 <= N) {
-        store4<false>(c + m * ldc + n, o);
-      } else {
-#pragma unroll
-        for (int r = 0; r < 4; ++r)
-          if (n + r < N) c[m * ldc + n + r] = o.v[r];
-      }
-    }
-  }
+  __syncthreads();  // every wave is done with the tiles
+  constexpr int ROOM = 2 * (TA::BYTES + TB::BYTES) / (WM * WN);
+  store_tile<T, O, WHOLE, FM, FN, ROOM>(acc, &lds[0][0] + wave * ROOM,
+                                        c + wm * ldc + wn, ldc, M - wm, N - wn);
 }
 
-__device__ inline int64_t offset_at(const int64_t* offsets, int g,
-                                    int64_t rows) {
+// offsets never change under a kernel: scalar loads, whatever it writes
+using ConstOffsets = const __attribute__((address_space(4))) int64_t*;
+
+__device__ inline int offset_at(ConstOffsets offsets, int g, int rows) {
   const int64_t o = offsets[g];
-  return o < 0 ? 0 : o > rows ? rows : o;  // never outside the rows
+  return o < 0 ? 0 : o > rows ? rows : (int)o;  // never outside the rows
+}
+
+// the tile of rows at virtual tile v: its group, first row and rows (0: none)
+struct Span {
+  int g, r0, many;
+};
+template <int BM>
+__device__ inline Span find_span(ConstOffsets offsets, int v, int rows, int G) {
+  int lo = 0, hi = G;  // the last g with start(g) <= v
+  while (hi - lo > 1) {
+    const int mid = (lo + hi) >> 1;
+    if (offset_at(offsets, mid, rows) / BM + mid <= v) lo = mid; else hi = mid;
+  }
+  const int begin = offset_at(offsets, lo, rows);
+  const int stop = offset_at(offsets, lo + 1, rows);
+  const int64_t r0 = begin + (int64_t)(v - begin / BM - lo) * BM;
+  if (r0 < begin || r0 >= stop) return {lo, 0, 0};
+  return {lo, (int)r0, min(BM, stop - (int)r0)};
+}
+
+template <typename T>
+__device__ inline void zero_outside(ConstOffsets offsets, T* y, int rows, int G,
+                                    int N) {
+  const int64_t first = offset_at(offsets, 0, rows);
+  const int64_t end = max((int)first, offset_at(offsets, G, rows));
+  const int64_t outside = (first + rows - end) * N;
+  for (int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; i < outside;
+       i += (int64_t)gridDim.x * blockDim.x)
+    y[i < first * N ? i : i + (end - first) * N] = (T)0.f;
 }
 
 // blocks go round robin over the 8 XCDs: neighbours in the work's order share
@@ -299,40 +385,287 @@ __device__ inline int64_t xcd_order(int64_t b, int64_t blocks) {
 template <typename T, bool WC, bool WHOLE, int BM, int BN, int WM, int WN>
 __global__ __launch_bounds__(64 * WM * WN) void segment_mm_kernel(
     const T* __restrict__ x, int64_t xs, const T* __restrict__ w, int64_t wg,
-    int64_t wl, const int64_t* __restrict__ offsets, T* __restrict__ y,
-    int64_t rows, int G, int K, int N, int tiles_n) {
-  // rows of no group
-  const int64_t first = offset_at(offsets, 0, rows);
-  const int64_t end = max(first, offset_at(offsets, G, rows));
-  const int64_t outside = (first + rows - end) * N;
-  for (int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; i < outside;
-       i += (int64_t)gridDim.x * blockDim.x)
-    y[i < first * N ? i : i + (end - first) * N] = (T)0.f;
-  const int64_t work = xcd_order(blockIdx.x, gridDim.x);
-  const int64_t v = work / tiles_n;
-  int lo = 0, hi = G;  // the last g with start(g) <= v
+    int64_t wl, ConstOffsets offsets, T* __restrict__ y, int rows, int G, int K,
+    int N, int tiles_n) {
+  zero_outside(offsets, y, rows, G, N);
+  const int work = (int)xcd_order(blockIdx.x, gridDim.x);
+  const Span s = find_span<BM>(offsets, work / tiles_n, rows, G);
+  if (s.many == 0) return;
+  const int n0 = work % tiles_n * BN;
+  tile_product<T, T, false, WC, WHOLE, BM, BN, WM, WN>(
+      x + s.r0 * xs, xs, s.many, w + s.g * wg + n0 * (WC ? 1 : wl), wl,
+      min(BN, N - n0), K, y + (int64_t)s.r0 * N + n0, N);
+}
+
+// ---------------------------------------------------------------------------
+// Many rows a group, 16-bit types: one block of 8 waves a CU walks over tiles of
+// 256 x 256. Steps of 64 bytes of depth go round a ring of 4 LDS stages: one is
+// multiplied from registers while the next is read into them and three more are
+// on their way; the loads run on into the next tile while this one's results go
+// out.
+// ---------------------------------------------------------------------------
+template <typename T, bool WC>
+__global__ __launch_bounds__(512) void segment_mm_wide_kernel(
+    const T* __restrict__ x, int64_t xs, const T* __restrict__ w, int64_t wg,
+    int64_t wl, ConstOffsets offsets, T* __restrict__ y, int rows, int G, int K,
+    int N, int tiles_n, int tiles) {
+  constexpr int B = 256, STEP = 64, STAGES = 4;
+  using TA = Tile<T, false, B, 512, STEP>;
+  using TB = Tile<T, WC, B, 512, STEP>;
+  constexpr int STAGE = TA::BYTES + TB::BYTES, BK = TA::BK;
+  constexpr int FM = 8, FN = 4, ROOM = 16 * (FN * 16 * sizeof(T) + 16);
+  __shared__ __align__(16) char lds[STAGES * STAGE + 8 * ROOM];
+  zero_outside(offsets, y, rows, G, N);
+  // an XCD's blocks walk side by side over its own stretch of the tiles
+  const int xcd = blockIdx.x & 7, t_step = gridDim.x >> 3;
+  const int t_end = (int)((int64_t)tiles * (xcd + 1) / 8);
+  auto next = [&](int t) {  // the first tile from t on that has rows
+    while (t < t_end && find_span<B>(offsets, t / tiles_n, rows, G).many == 0)
+      t += t_step;
+    return t;
+  };
+  int use_t = next((int)((int64_t)tiles * xcd / 8) + (blockIdx.x >> 3));
+  if (use_t >= t_end) return;
+  int load_t = use_t, load_left = K;
+  const T* a;
+  const T* b;
+  uint32_t pa[TA::PER], pb[TB::PER];
+  auto enter = [&](int t) {
+    const Span s = find_span<B>(offsets, t / tiles_n, rows, G);
+    const int n0 = t % tiles_n * B;
+    a = x + s.r0 * xs;
+    b = w + s.g * wg + n0 * (WC ? 1 : wl);
+    TA::place(xs, s.many, pa);
+    TB::place(wl, min(B, N - n0), pb);
+  };
+  enter(load_t);
+  const int64_t step_b = WC ? BK * wl : BK;
+  auto ahead = [&](char* stage) {
+    TA::load(a, pa, load_left, stage);
+    TB::load(b, pb, load_left, stage + TA::BYTES);
+    a += BK;
+    b += step_b;
+    load_left -= BK;
+    if (load_left > 0) return;
+    load_left = K;
+    load_t = load_t < t_end ? next(load_t + t_step) : t_end;
+    if (load_t < t_end) {
+      enter(load_t);
+    } else {
+      // behind the last tile the loads go on out of range, so that a wait's
+      // count always means the same
+      TA::place(xs, 0, pa);
+      TB::place(wl, 0, pb);
+    }
+  };
+#pragma unroll 1
+  for (int i = 0; i < STAGES; ++i) ahead(lds + i * STAGE);
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int wm = wave / 4 * 128, wn = wave % 4 * 64;
+  const typename TA::template Reader<FM> read_a(wm);
+  const typename TB::template Reader<FN> read_b(wn);
+  static_assert(TA::PER + TB::PER == 4, "the waits count loads");
+  typename TA::Frag fa[FM];
+  typename TB::Frag fb[FN];
+  asm volatile("s_waitcnt vmcnt(12)\n\ts_barrier" ::: "memory");
+#pragma unroll
+  for (int j = 0; j < FN; ++j) fb[j] = read_b.get(lds + TA::BYTES, j, 0);
+#pragma unroll
+  for (int i = 0; i < FM; ++i) fa[i] = read_a.get(lds, i, 0);
+  int stage = 0;
+  while (use_t < t_end) {
+    f32x4 acc[FM][FN] = {};
+#pragma unroll 1
+    for (int left = K; left > 0; left -= BK) {
+      // The fragments of this step are in registers, the next stage has arrived
+      // and two are on their way; every wave has read this stage, which the
+      // loads may fill again. The next step's fragments replace this one's as
+      // these are used up.
+      asm volatile("s_waitcnt vmcnt(8) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+      ahead(lds + stage * STAGE);
+      stage = (stage + 1) & (STAGES - 1);
+      const char* la = lds + stage * STAGE;
+      typename TB::Frag nb[FN];
+#pragma unroll
+      for (int j = 0; j < FN; ++j) nb[j] = read_b.get(la + TA::BYTES, j, 0);
+#pragma unroll
+      for (int i = 0; i < FM; ++i) {
+#pragma unroll
+        for (int j = 0; j < FN; ++j)
+          acc[i][j] = mma<T>(fb[j], fa[i], acc[i][j]);
+        fa[i] = read_a.get(la, i, 0);
+      }
+#pragma unroll
+      for (int j = 0; j < FN; ++j) fb[j] = nb[j];
+    }
+    const Span s = find_span<B>(offsets, use_t / tiles_n, rows, G);
+    const int n0 = use_t % tiles_n * B;
+    store_tile<T, T, true, FM, FN, ROOM>(
+        acc, lds + STAGES * STAGE + wave * ROOM,
+        y + (int64_t)(s.r0 + wm) * N + n0 + wn, N, s.many - wm, N - n0 - wn);
+    use_t = next(use_t + t_step);
+  }
+  // nothing may still be on its way into LDS when the block ends
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+}
+
+// dW over many rows a group, 16-bit types, the same ring. The rows of all groups
+// are dealt evenly to teams, a team being one block for each 256 x 256 tile of
+// a group's dW (they read the same rows, on one XCD where they fit). A block
+// walks over its team's rows; where they hold a whole group its product goes
+// straight to dW, where they begin or end inside one it goes to the team's
+// first or second fp32 plane, and sum_teams_kernel adds those up.
+struct Team {
+  int begin, each;  // the first row of all, rows a team
+};
+__device__ inline Team team_rows(ConstOffsets offsets, int rows, int G,
+                                 int teams) {
+  const int first = offset_at(offsets, 0, rows);
+  const int all = max(0, offset_at(offsets, G, rows) - first);
+  return {first, max(32, ((all + teams - 1) / teams + 31) & ~31)};
+}
+
+template <typename T>
+__global__ __launch_bounds__(512) void segment_wgrad_wide_kernel(
+    const T* __restrict__ x, int64_t xs, const T* __restrict__ g, int64_t gs,
+    ConstOffsets offsets, T* __restrict__ dw, float* __restrict__ planes,
+    int rows, int G, int K, int N, int tiles_n, int tiles, int teams) {
+  constexpr int B = 256, STEP = 64, STAGES = 4;
+  using TT = Tile<T, true, B, 512, STEP>;
+  constexpr int STAGE = 2 * TT::BYTES, BK = TT::BK;
+  constexpr int FM = 8, FN = 4, ROOM = 16 * (FN * 16 * sizeof(T) + 16);
+  __shared__ __align__(16) char lds[STAGES * STAGE + 8 * ROOM];
+  const int id = (blockIdx.x & 7) * (gridDim.x >> 3) + (blockIdx.x >> 3);
+  const int team = id / tiles, tile = id % tiles;
+  if (team >= teams) return;
+  const int k0 = tile / tiles_n * B, n0 = tile % tiles_n * B;
+  const Team tr = team_rows(offsets, rows, G, teams);
+  const int from = tr.begin + (int)min((int64_t)team * tr.each, (int64_t)rows);
+  const int to = (int)min((int64_t)from + tr.each,
+                          (int64_t)offset_at(offsets, G, rows));
+  if (from >= to) return;
+  auto stop_of = [&](int e) { return min(to, offset_at(offsets, e + 1, rows)); };
+  // the group that holds row r >= its start: the first from e on that ends later
+  auto group_of = [&](int e, int r) {
+    while (e < G - 1 && offset_at(offsets, e + 1, rows) <= r) ++e;
+    return e;
+  };
+  int lo = 0, hi = G;  // the last group that starts at or before `from`
   while (hi - lo > 1) {
     const int mid = (lo + hi) >> 1;
-    if (offset_at(offsets, mid, rows) / BM + mid <= v) lo = mid; else hi = mid;
+    if (offset_at(offsets, mid, rows) <= from) lo = mid; else hi = mid;
   }
-  const int64_t begin = offset_at(offsets, lo, rows);
-  const int64_t r0 = begin + (v - begin / BM - lo) * BM;
-  const int64_t stop = offset_at(offsets, lo + 1, rows);
-  if (r0 < begin || r0 >= stop) return;
-  const int n0 = (int)(work % tiles_n) * BN;
-  tile_product<T, T, false, WC, WHOLE, BM, BN, WM, WN>(
-      x + r0 * xs, xs, (int)min((int64_t)BM, stop - r0),
-      w + lo * wg + n0 * (WC ? 1 : wl), wl, min(BN, N - n0), K,
-      y + r0 * N + n0, N);
+  int use_g = lo, use_r = from, load_g = lo, load_r = from;
+  int load_stop = max(from + 1, stop_of(lo));
+  uint32_t pa[TT::PER], pb[TT::PER];
+  TT::place(xs, min(B, K - k0), pa);
+  TT::place(gs, min(B, N - n0), pb);
+  auto ahead = [&](char* stage) {
+    const int depth = load_stop - load_r;  // 0 behind the last row: no loads
+    TT::load(x + load_r * xs + k0, pa, depth, stage);
+    TT::load(g + load_r * gs + n0, pb, depth, stage + TT::BYTES);
+    load_r = min(load_stop, load_r + BK);
+    if (load_r < load_stop || load_r >= to) return;
+    load_g = group_of(load_g, load_r);
+    load_stop = max(load_r + 1, stop_of(load_g));
+  };
+#pragma unroll 1
+  for (int i = 0; i < STAGES; ++i) ahead(lds + i * STAGE);
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int wm = wave / 4 * 128, wn = wave % 4 * 64;
+  const typename TT::template Reader<FM> read_a(wm);
+  const typename TT::template Reader<FN> read_b(wn);
+  static_assert(2 * TT::PER == 4, "the waits count loads");
+  typename TT::Frag fa[FM], fb[FN];
+  asm volatile("s_waitcnt vmcnt(12)\n\ts_barrier" ::: "memory");
+#pragma unroll
+  for (int j = 0; j < FN; ++j) fb[j] = read_b.get(lds + TT::BYTES, j, 0);
+#pragma unroll
+  for (int i = 0; i < FM; ++i) fa[i] = read_a.get(lds, i, 0);
+  int stage = 0;
+  while (use_r < to) {
+    f32x4 acc[FM][FN] = {};
+    const int start = use_r, stop = max(use_r + 1, stop_of(use_g));
+#pragma unroll 1
+    for (int left = stop - start; left > 0; left -= BK) {
+      asm volatile("s_waitcnt vmcnt(8) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+      ahead(lds + stage * STAGE);
+      stage = (stage + 1) & (STAGES - 1);
+      const char* la = lds + stage * STAGE;
+      typename TT::Frag nb[FN];
+#pragma unroll
+      for (int j = 0; j < FN; ++j) nb[j] = read_b.get(la + TT::BYTES, j, 0);
+#pragma unroll
+      for (int i = 0; i < FM; ++i) {
+#pragma unroll
+        for (int j = 0; j < FN; ++j)
+          acc[i][j] = mma<T>(fb[j], fa[i], acc[i][j]);
+        fa[i] = read_a.get(la, i, 0);
+      }
+#pragma unroll
+      for (int j = 0; j < FN; ++j) fb[j] = nb[j];
+    }
+    const int M = K - k0 - wm, W = N - n0 - wn;
+    const int64_t corner = (int64_t)(k0 + wm) * N + n0 + wn;
+    const int g_start = offset_at(offsets, use_g, rows);
+    const int g_stop = offset_at(offsets, use_g + 1, rows);
+    if (start == g_start && stop == g_stop) {
+      store_tile<T, T, true, FM, FN, ROOM>(
+          acc, lds + STAGES * STAGE + wave * ROOM,
+          dw + (int64_t)use_g * K * N + corner, N, M, W);
+    } else {
+      // begun in an earlier team: the first plane, else the second
+      float* c = planes + (2 * (int64_t)team + (start == g_start)) * K * N + corner;
+      const int lane = thread_here() & 63;
+#pragma unroll
+      for (int i = 0; i < FM; ++i)
+#pragma unroll
+        for (int j = 0; j < FN; ++j) {
+          const int m = i * 16 + (lane & 15), n = j * 16 + (lane >> 4) * 4;
+          if (m < M && n < W)
+            *reinterpret_cast<f32x4*>(c + (int64_t)m * N + n) = acc[i][j];
+        }
+    }
+    use_r = stop;
+    if (use_r < to) use_g = group_of(use_g, use_r);
+  }
+  // nothing may still be on its way into LDS when the block ends
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+}
+
+// groups that several teams hold, the teams in order; empty groups
+template <typename T>
+__global__ __launch_bounds__(256) void sum_teams_kernel(
+    const float* __restrict__ planes, ConstOffsets offsets, T* __restrict__ dw,
+    int rows, int G, int64_t n, int teams) {
+  const int e = blockIdx.y;
+  const int b = offset_at(offsets, e, rows), s = offset_at(offsets, e + 1, rows);
+  const Team tr = team_rows(offsets, rows, G, teams);
+  // (clamped for offsets that fall: the planes are never left)
+  const int t0 = min(teams - 1, max(0, b - tr.begin) / tr.each);
+  const int t1 = min(teams - 1, max(0, s - 1 - tr.begin) / tr.each);
+  if (s > b && t0 == t1) return;  // whole in one team
+  for (int64_t i = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 4; i < n;
+       i += (int64_t)gridDim.x * 1024) {
+    f32x4 sum = {};
+    if (s > b)
+      for (int t = t0; t <= t1; ++t)
+        sum += *reinterpret_cast<const f32x4*>(
+            planes + (2 * (int64_t)t + (t == t0)) * n + i);
+    Vec<T, 4> o;
+#pragma unroll
+    for (int r = 0; r < 4; ++r) o.v[r] = (T)sum[r];
+    *reinterpret_cast<Vec<T, 4>*>(dw + e * n + i) = o;
+  }
 }
 
 // dW tiles; the group's rows in `splits` parts, each to its own plane of `out`
 template <typename T, typename O, bool WHOLE, int BM, int BN, int WM, int WN>
 __global__ __launch_bounds__(64 * WM * WN) void segment_mm_wgrad_kernel(
     const T* __restrict__ x, int64_t xs, const T* __restrict__ g, int64_t gs,
-    const int64_t* __restrict__ offsets, O* __restrict__ out, int64_t rows,
-    int G, int K, int N, int tiles_k, int tiles_n, int splits) {
-  int64_t work = xcd_order(blockIdx.x, gridDim.x);
+    ConstOffsets offsets, O* __restrict__ out, int rows, int G, int K, int N,
+    int tiles_k, int tiles_n, int splits) {
+  int work = (int)xcd_order(blockIdx.x, gridDim.x);
   const int n0 = (int)(work % tiles_n) * BN;
   work /= tiles_n;
   const int k0 = (int)(work % tiles_k) * BM;
@@ -340,7 +673,7 @@ __global__ __launch_bounds__(64 * WM * WN) void segment_mm_wgrad_kernel(
   const int part = (int)(work % splits);
   const int e = (int)(work / splits);
   const int64_t begin = offset_at(offsets, e, rows);
-  const int64_t len = max((int64_t)0, offset_at(offsets, e + 1, rows) - begin);
+  const int64_t len = max(0, offset_at(offsets, e + 1, rows) - (int)begin);
   constexpr int BK = kStepBytes / sizeof(T);
   const int64_t each = (len + (int64_t)splits * BK - 1) / (splits * BK) * BK;
   const int64_t from = min(len, part * each), to = min(len, from + each);
@@ -393,6 +726,16 @@ static void check_offsets(const at::Tensor& offsets, const at::Tensor& x,
   TORCH_CHECK(groups <= 65535, what, ": at most 65535 groups");
 }
 
+// blocks of a kernel that fills the chip once: a multiple of the 8 XCDs
+static int cu_count() {
+  static const int cus = [] {
+    hipDeviceProp_t p;
+    DOA_CHECK_HIP(hipGetDeviceProperties(&p, 0));
+    return std::max(8, p.multiProcessorCount / 8 * 8);
+  }();
+  return cus;
+}
+
 // whether a tile of rows can be read in whole aligned chunks, from byte offsets
 // below 2^31
 template <typename T>
@@ -425,6 +768,8 @@ at::Tensor segment_mm(at::Tensor offsets, at::Tensor x, at::Tensor weight,
   c10::DeviceGuard guard(x.device());
   auto xc = mm_rows(x);
   const int64_t R = x.size(0);
+  TORCH_CHECK(R < (1 << 30), "segment_mm: too many rows");
+  const auto op = (ConstOffsets)offsets.data_ptr<int64_t>();
   auto y = at::empty({R, N}, x.options());
   if (R * N == 0) return y;
   // one of the weight's two inner strides has to be 1
@@ -439,14 +784,27 @@ at::Tensor segment_mm(at::Tensor offsets, at::Tensor x, at::Tensor weight,
       hipLaunchKernelGGL(kernel, dim3(blocks), dim3(threads), 0,
                          stream_of_current(), (const T*)xc.data_ptr(),
                          xc.stride(0), (const T*)wt.data_ptr(), wt.stride(0),
-                         wl, offsets.data_ptr<int64_t>(), (T*)y.data_ptr(), R,
-                         (int)G, (int)K, (int)N, (int)tn);
+                         wl, op, (T*)y.data_ptr(), (int)R, (int)G, (int)K,
+                         (int)N, (int)tn);
     };
     // whole aligned chunks of 16 bytes go straight to LDS
     const bool whole = whole_rows<T>(xc, K) && N % (16 / sizeof(T)) == 0 &&
                        K % (16 / sizeof(T)) == 0 && whole_weight<T>(wt, wl);
     auto pick = [&](auto wcv, auto wv) {
       constexpr bool WC = decltype(wcv)::value, W = decltype(wv)::value;
+      if constexpr (W && sizeof(T) == 2) {
+        if (N >= 256 && R >= 512 * G && K > 0) {
+          const int64_t tn = ceil_div(N, 256), tiles = (R / 256 + G) * tn;
+          TORCH_CHECK(tiles < (1 << 30), "segment_mm: too many tiles");
+          hipLaunchKernelGGL((segment_mm_wide_kernel<T, WC>), dim3(cu_count()),
+                             dim3(512), 0, stream_of_current(),
+                             (const T*)xc.data_ptr(), xc.stride(0),
+                             (const T*)wt.data_ptr(), wt.stride(0), wl,
+                             op, (T*)y.data_ptr(), (int)R, (int)G, (int)K, (int)N,
+                             (int)tn, (int)tiles);
+          return;
+        }
+      }
       // few rows a group: a tile of 32 rows leaves less of it empty and reads
       // the weights over more blocks
       if (R <= 48 * G)
@@ -478,6 +836,7 @@ at::Tensor segment_mm_wgrad(at::Tensor offsets, at::Tensor x, at::Tensor grad) {
   auto xc = mm_rows(x);
   auto gc = mm_rows(grad);
   const int64_t K = x.size(1), N = grad.size(1), R = x.size(0);
+  TORCH_CHECK(R < (1 << 30), "segment_mm: too many rows");
   auto dw = at::empty({G, K, N}, x.options());
   if (dw.numel() == 0) return dw;
   constexpr int B = 128;
@@ -488,6 +847,28 @@ at::Tensor segment_mm_wgrad(at::Tensor offsets, at::Tensor x, at::Tensor grad) {
   TORCH_CHECK(tiles * splits < INT32_MAX, "segment_mm: too many tiles");
   DOA_FLOAT_TYPES(x.scalar_type(), "segment_mm", [&] {
     const bool whole = whole_rows<T>(xc, K) && whole_rows<T>(gc, N);
+    if constexpr (sizeof(T) == 2) {
+      const int cus = cu_count();
+      const int64_t wn = ceil_div(N, 256), wide = ceil_div(K, 256) * wn;
+      if (whole && K >= 128 && N >= 128 && R >= 512 * G && wide <= cus) {
+        const int teams = (int)(cus / wide);
+        auto planes = at::empty({2 * teams * K * N},
+                                x.options().dtype(at::kFloat));
+        const auto op = (ConstOffsets)offsets.data_ptr<int64_t>();
+        hipLaunchKernelGGL((segment_wgrad_wide_kernel<T>), dim3(cus), dim3(512),
+                           0, stream_of_current(), (const T*)xc.data_ptr(),
+                           xc.stride(0), (const T*)gc.data_ptr(), gc.stride(0),
+                           op, (T*)dw.data_ptr(), planes.data_ptr<float>(),
+                           (int)R, (int)G, (int)K, (int)N, (int)wn, (int)wide,
+                           teams);
+        hipLaunchKernelGGL((sum_teams_kernel<T>),
+                           dim3(grid_for(ceil_div(K * N, 4), 256, 1024), G),
+                           dim3(256), 0, stream_of_current(),
+                           planes.data_ptr<float>(), op, (T*)dw.data_ptr(),
+                           (int)R, (int)G, K * N, teams);
+        return;
+      }
+    }
     auto go = [&](auto* out) {
       using O = std::remove_pointer_t<decltype(out)>;
       auto kernel = whole ? segment_mm_wgrad_kernel<T, O, true, B, B, 2, 2>
@@ -495,8 +876,8 @@ at::Tensor segment_mm_wgrad(at::Tensor offsets, at::Tensor x, at::Tensor grad) {
       hipLaunchKernelGGL(kernel, dim3(tiles * splits), dim3(256), 0,
                          stream_of_current(), (const T*)xc.data_ptr(),
                          xc.stride(0), (const T*)gc.data_ptr(), gc.stride(0),
-                         offsets.data_ptr<int64_t>(), out, R, (int)G, (int)K,
-                         (int)N, (int)tk, (int)tn, (int)splits);
+                         (ConstOffsets)offsets.data_ptr<int64_t>(), out, (int)R,
+                         (int)G, (int)K, (int)N, (int)tk, (int)tn, (int)splits);
     };
     if (splits == 1) {
       go((T*)dw.data_ptr());

@@ -185,6 +185,9 @@ SHAPES = [
     ([700, 300, 24], 512, 136, 0, 0),
     ([40] * 30, 72, 40, 0, 0),
     ([5000], 16, 16, 0, 0),
+    ([2100, 0, 520], 136, 264, 0, 2),
+    ([1100], 264, 320, 1, 0),
+    ([0, 700, 0, 3300, 1, 0], 256, 520, 40, 9),
 ]
 
 

@@ -251,29 +251,35 @@ __device__ inline void store_tile(const f32x4 (&acc)[FM][FN], char* room, O* c,
   }
 }
 
+// two stages of both operands
+constexpr int lds_bytes(int BM, int BN) { return 2 * (BM + BN) * kStepBytes; }
+
 // c[m][n] = sum_k a(m, k) b(k, n) for one tile of BM x BN. AC, BC: that
 // operand's depth is its outer index. WM x WN waves. WHOLE: every row of both
 // starts on 16 bytes and is whole chunks long.
 template <typename T, typename O, bool AC, bool BC, bool WHOLE, int BM, int BN,
           int WM, int WN>
-__device__ inline void tile_product(const T* a, int64_t lda, int M, const T* b,
-                                    int64_t ldb, int N, int64_t K, O* c,
-                                    int64_t ldc) {
+__device__ inline void tile_product(char* lds, const T* a, int64_t lda, int M,
+                                    const T* b, int64_t ldb, int N, int64_t K,
+                                    O* c, int64_t ldc) {
   constexpr int THREADS = 64 * WM * WN;
   using TA = Tile<T, AC, BM, THREADS>;
   using TB = Tile<T, BC, BN, THREADS>;
   constexpr int FM = BM / WM / 16, FN = BN / WN / 16;
   constexpr int BK = TA::BK;
-  __shared__ __align__(16) char lds[2][TA::BYTES + TB::BYTES];
+  constexpr int STAGE = TA::BYTES + TB::BYTES;
+  static_assert(2 * STAGE == lds_bytes(BM, BN), "LDS");
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int wm = wave / WN * (BM / WM), wn = wave % WN * (BN / WN);
   const typename TA::template Reader<FM> read_a(wm);
   const typename TB::template Reader<FN> read_b(wn);
   f32x4 acc[FM][FN] = {};
   const int64_t step_a = AC ? BK * lda : BK, step_b = BC ? BK * ldb : BK;
-  auto multiply = [&](const char* la, const char* lb) {
+  auto multiply = [&](const char* la, const char* lb, int64_t left) {
 #pragma unroll
     for (int kk = 0; kk < 2; ++kk) {
+      // fp32's matrix rate is worth a branch around zeros
+      if (sizeof(T) == 4 && kk && left <= BK / 2) continue;
       typename TA::Frag fa[FM];
       typename TB::Frag fb[FN];
 #pragma unroll
@@ -294,8 +300,8 @@ __device__ inline void tile_product(const T* a, int64_t lda, int M, const T* b,
     TA::place(lda, M, pa);
     TB::place(ldb, N, pb);
     if (K > 0) {
-      TA::load(a, pa, K, lds[0]);
-      TB::load(b, pb, K, lds[0] + TA::BYTES);
+      TA::load(a, pa, K, lds);
+      TB::load(b, pb, K, lds + TA::BYTES);
     }
     for (int64_t left = K; left > 0; left -= BK, now ^= 1) {
       // this step has arrived, and the last one's readers are done
@@ -304,18 +310,18 @@ __device__ inline void tile_product(const T* a, int64_t lda, int M, const T* b,
       if (left > BK) {  // the next step travels while this one multiplies
         a += step_a;
         b += step_b;
-        TA::load(a, pa, left - BK, lds[now ^ 1]);
-        TB::load(b, pb, left - BK, lds[now ^ 1] + TA::BYTES);
+        TA::load(a, pa, left - BK, lds + (now ^ 1) * STAGE);
+        TB::load(b, pb, left - BK, lds + (now ^ 1) * STAGE + TA::BYTES);
       }
-      multiply(lds[now], lds[now] + TA::BYTES);
+      multiply(lds + now * STAGE, lds + now * STAGE + TA::BYTES, left);
     }
   } else {
     Chunk ra[TA::PER], rb[TB::PER];
     if (K > 0) {
       TA::fetch(a, lda, M, K, ra);
       TB::fetch(b, ldb, N, K, rb);
-      TA::put(ra, lds[0]);
-      TB::put(rb, lds[0] + TA::BYTES);
+      TA::put(ra, lds);
+      TB::put(rb, lds + TA::BYTES);
     }
     for (int64_t left = K; left > 0; left -= BK, now ^= 1) {
       __syncthreads();
@@ -325,16 +331,16 @@ __device__ inline void tile_product(const T* a, int64_t lda, int M, const T* b,
         TA::fetch(a, lda, M, left - BK, ra);
         TB::fetch(b, ldb, N, left - BK, rb);
       }
-      multiply(lds[now], lds[now] + TA::BYTES);
+      multiply(lds + now * STAGE, lds + now * STAGE + TA::BYTES, left);
       if (left > BK) {
-        TA::put(ra, lds[now ^ 1]);
-        TB::put(rb, lds[now ^ 1] + TA::BYTES);
+        TA::put(ra, lds + (now ^ 1) * STAGE);
+        TB::put(rb, lds + (now ^ 1) * STAGE + TA::BYTES);
       }
     }
   }
   __syncthreads();  // every wave is done with the tiles
-  constexpr int ROOM = 2 * (TA::BYTES + TB::BYTES) / (WM * WN);
-  store_tile<T, O, WHOLE, FM, FN, ROOM>(acc, &lds[0][0] + wave * ROOM,
+  constexpr int ROOM = 2 * STAGE / (WM * WN);
+  store_tile<T, O, WHOLE, FM, FN, ROOM>(acc, lds + wave * ROOM,
                                         c + wm * ldc + wn, ldc, M - wm, N - wn);
 }
 
@@ -383,17 +389,18 @@ __device__ inline int64_t xcd_order(int64_t b, int64_t blocks) {
 }
 
 template <typename T, bool WC, bool WHOLE, int BM, int BN, int WM, int WN>
-__global__ __launch_bounds__(64 * WM * WN) void segment_mm_kernel(
+__global__ __launch_bounds__(64 * WM * WN, 2) void segment_mm_kernel(
     const T* __restrict__ x, int64_t xs, const T* __restrict__ w, int64_t wg,
     int64_t wl, ConstOffsets offsets, T* __restrict__ y, int rows, int G, int K,
     int N, int tiles_n) {
   zero_outside(offsets, y, rows, G, N);
   const int work = (int)xcd_order(blockIdx.x, gridDim.x);
+  __shared__ __align__(16) char lds[lds_bytes(BM, BN)];
   const Span s = find_span<BM>(offsets, work / tiles_n, rows, G);
   if (s.many == 0) return;
   const int n0 = work % tiles_n * BN;
   tile_product<T, T, false, WC, WHOLE, BM, BN, WM, WN>(
-      x + s.r0 * xs, xs, s.many, w + s.g * wg + n0 * (WC ? 1 : wl), wl,
+      lds, x + s.r0 * xs, xs, s.many, w + s.g * wg + n0 * (WC ? 1 : wl), wl,
       min(BN, N - n0), K, y + (int64_t)s.r0 * N + n0, N);
 }
 
@@ -647,66 +654,78 @@ __global__ __launch_bounds__(256) void sum_teams_kernel(
   if (s > b && t0 == t1) return;  // whole in one team
   for (int64_t i = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 4; i < n;
        i += (int64_t)gridDim.x * 1024) {
-    f32x4 sum = {};
-    if (s > b)
-      for (int t = t0; t <= t1; ++t)
-        sum += *reinterpret_cast<const f32x4*>(
-            planes + (2 * (int64_t)t + (t == t0)) * n + i);
-    Vec<T, 4> o;
+    if (n % 4 == 0) {
+      f32x4 sum = {};
+      if (s > b)
+        for (int t = t0; t <= t1; ++t)
+          sum += *reinterpret_cast<const f32x4*>(
+              planes + (2 * (int64_t)t + (t == t0)) * n + i);
+      Vec<T, 4> o;
 #pragma unroll
-    for (int r = 0; r < 4; ++r) o.v[r] = (T)sum[r];
-    *reinterpret_cast<Vec<T, 4>*>(dw + e * n + i) = o;
+      for (int r = 0; r < 4; ++r) o.v[r] = (T)sum[r];
+      *reinterpret_cast<Vec<T, 4>*>(dw + e * n + i) = o;
+    } else {
+      for (int64_t j = i; j < min(n, i + 4); ++j) {
+        float sum = 0.f;
+        if (s > b)
+          for (int t = t0; t <= t1; ++t)
+            sum += planes[(2 * (int64_t)t + (t == t0)) * n + j];
+        dw[e * n + j] = (T)sum;
+      }
+    }
   }
 }
 
-// dW tiles; the group's rows in `splits` parts, each to its own plane of `out`
-template <typename T, typename O, bool WHOLE, int BM, int BN, int WM, int WN>
-__global__ __launch_bounds__(64 * WM * WN) void segment_mm_wgrad_kernel(
+// dW by a block for each group and tile: many groups
+template <typename T, bool WHOLE, int BM, int BN, int WM, int WN>
+__global__ __launch_bounds__(64 * WM * WN, 2) void segment_wgrad_kernel(
     const T* __restrict__ x, int64_t xs, const T* __restrict__ g, int64_t gs,
-    ConstOffsets offsets, O* __restrict__ out, int rows, int G, int K, int N,
-    int tiles_k, int tiles_n, int splits) {
+    ConstOffsets offsets, T* __restrict__ dw, int rows, int K, int N,
+    int tiles_k, int tiles_n) {
+  __shared__ __align__(16) char lds[lds_bytes(BM, BN)];
   int work = (int)xcd_order(blockIdx.x, gridDim.x);
-  const int n0 = (int)(work % tiles_n) * BN;
+  const int n0 = work % tiles_n * BN;
   work /= tiles_n;
-  const int k0 = (int)(work % tiles_k) * BM;
-  work /= tiles_k;
-  const int part = (int)(work % splits);
-  const int e = (int)(work / splits);
+  const int k0 = work % tiles_k * BM, e = work / tiles_k;
   const int64_t begin = offset_at(offsets, e, rows);
-  const int64_t len = max(0, offset_at(offsets, e + 1, rows) - (int)begin);
-  constexpr int BK = kStepBytes / sizeof(T);
-  const int64_t each = (len + (int64_t)splits * BK - 1) / (splits * BK) * BK;
-  const int64_t from = min(len, part * each), to = min(len, from + each);
-  tile_product<T, O, true, true, WHOLE, BM, BN, WM, WN>(
-      x + (begin + from) * xs + k0, xs, min(BM, K - k0),
-      g + (begin + from) * gs + n0, gs, min(BN, N - n0), to - from,
-      out + (((int64_t)part * G + e) * K + k0) * N + n0, N);
+  const int64_t len = offset_at(offsets, e + 1, rows) - begin;
+  tile_product<T, T, true, true, WHOLE, BM, BN, WM, WN>(
+      lds, x + begin * xs + k0, xs, min(BM, K - k0), g + begin * gs + n0, gs,
+      min(BN, N - n0), len, dw + ((int64_t)e * K + k0) * N + n0, N);
 }
 
-// the parts' sum, in their order
-template <typename T>
-__global__ __launch_bounds__(256) void sum_parts_kernel(
-    const float* __restrict__ parts, T* __restrict__ out, int64_t n,
-    int splits) {
-  for (int64_t i = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 4; i < n;
-       i += (int64_t)gridDim.x * 1024) {
-    if (i + 4 <= n) {
-      float s[4] = {};
-      for (int p = 0; p < splits; ++p) {
-        union { Chunk q; float v[4]; } u;
-        u.q = *reinterpret_cast<const LooseChunk*>(parts + p * n + i);
-#pragma unroll
-        for (int e = 0; e < 4; ++e) s[e] += u.v[e];
-      }
-#pragma unroll
-      for (int e = 0; e < 4; ++e) out[i + e] = (T)s[e];
-    } else {
-      for (int64_t j = i; j < n; ++j) {
-        float s = 0.f;
-        for (int p = 0; p < splits; ++p) s += parts[p * n + j];
-        out[j] = (T)s;
-      }
-    }
+// dW by teams, as segment_wgrad_wide_kernel: few groups with many rows
+template <typename T, bool WHOLE, int BM, int BN, int WM, int WN>
+__global__ __launch_bounds__(64 * WM * WN, 2) void segment_wgrad_teams_kernel(
+    const T* __restrict__ x, int64_t xs, const T* __restrict__ g, int64_t gs,
+    ConstOffsets offsets, T* __restrict__ dw, float* __restrict__ planes,
+    int rows, int G, int K, int N, int tiles_n, int tiles, int teams) {
+  const int work = (int)xcd_order(blockIdx.x, gridDim.x);
+  __shared__ __align__(16) char lds[lds_bytes(BM, BN)];
+  const int team = work / tiles, tile = work % tiles;
+  const int k0 = tile / tiles_n * BM, n0 = tile % tiles_n * BN;
+  const Team tr = team_rows(offsets, rows, G, teams);
+  const int from = tr.begin + (int)min((int64_t)team * tr.each, (int64_t)rows);
+  const int to = (int)min((int64_t)from + tr.each,
+                          (int64_t)offset_at(offsets, G, rows));
+  for (int r = from, e = 0; r < to;) {
+    while (e < G - 1 && offset_at(offsets, e + 1, rows) <= r) ++e;
+    const int g_start = offset_at(offsets, e, rows);
+    const int g_stop = offset_at(offsets, e + 1, rows);
+    const int stop = max(r + 1, min(to, g_stop));
+    const T* a = x + r * xs + k0;
+    const T* b = g + r * gs + n0;
+    const int64_t corner = (int64_t)k0 * N + n0;
+    __syncthreads();  // the last product's LDS is free
+    if (r == g_start && stop == g_stop)
+      tile_product<T, T, true, true, WHOLE, BM, BN, WM, WN>(
+          lds, a, xs, min(BM, K - k0), b, gs, min(BN, N - n0), stop - r,
+          dw + (int64_t)e * K * N + corner, N);
+    else
+      tile_product<T, float, true, true, WHOLE, BM, BN, WM, WN>(
+          lds, a, xs, min(BM, K - k0), b, gs, min(BN, N - n0), stop - r,
+          planes + (2 * (int64_t)team + (r == g_start)) * K * N + corner, N);
+    r = stop;
   }
 }
 
@@ -809,6 +828,8 @@ at::Tensor segment_mm(at::Tensor offsets, at::Tensor x, at::Tensor weight,
       // the weights over more blocks
       if (R <= 48 * G)
         go(segment_mm_kernel<T, WC, W, 32, 64, 1, 4>, 32, 64, 256);
+      else if constexpr (sizeof(T) == 4)
+        go(segment_mm_kernel<T, WC, W, 64, 64, 2, 2>, 64, 64, 256);
       else
         go(segment_mm_kernel<T, WC, W, 128, 128, 2, 2>, 128, 128, 256);
     };
@@ -839,58 +860,53 @@ at::Tensor segment_mm_wgrad(at::Tensor offsets, at::Tensor x, at::Tensor grad) {
   TORCH_CHECK(R < (1 << 30), "segment_mm: too many rows");
   auto dw = at::empty({G, K, N}, x.options());
   if (dw.numel() == 0) return dw;
-  constexpr int B = 128;
-  const int64_t tk = ceil_div(K, B), tn = ceil_div(N, B), tiles = G * tk * tn;
-  // few tiles over long groups: parts of at least 512 rows, about 1024 blocks
-  const int64_t splits = std::max<int64_t>(
-      1, std::min<int64_t>({ceil_div(1024, tiles), R / G / 512, 64}));
-  TORCH_CHECK(tiles * splits < INT32_MAX, "segment_mm: too many tiles");
   DOA_FLOAT_TYPES(x.scalar_type(), "segment_mm", [&] {
     const bool whole = whole_rows<T>(xc, K) && whole_rows<T>(gc, N);
+    const T* xp = (const T*)xc.data_ptr();
+    const T* gp = (const T*)gc.data_ptr();
+    const auto op = (ConstOffsets)offsets.data_ptr<int64_t>();
+    const auto stream = stream_of_current();
+    const int cus = cu_count();
+    at::Tensor planes;
+    auto by_teams = [&](auto kernel, int blocks, int threads, int BN,
+                        int64_t tiles, int teams) {
+      planes = at::empty({2 * teams * K * N}, x.options().dtype(at::kFloat));
+      hipLaunchKernelGGL(kernel, dim3(blocks), dim3(threads), 0, stream, xp,
+                         xc.stride(0), gp, gc.stride(0), op, (T*)dw.data_ptr(),
+                         planes.data_ptr<float>(), (int)R, (int)G, (int)K,
+                         (int)N, (int)ceil_div(N, BN), (int)tiles, teams);
+      hipLaunchKernelGGL((sum_teams_kernel<T>),
+                         dim3(grid_for(ceil_div(K * N, 4), 256, 1024), G),
+                         dim3(256), 0, stream, planes.data_ptr<float>(), op,
+                         (T*)dw.data_ptr(), (int)R, (int)G, K * N, teams);
+    };
     if constexpr (sizeof(T) == 2) {
-      const int cus = cu_count();
-      const int64_t wn = ceil_div(N, 256), wide = ceil_div(K, 256) * wn;
-      if (whole && K >= 128 && N >= 128 && R >= 512 * G && wide <= cus) {
-        const int teams = (int)(cus / wide);
-        auto planes = at::empty({2 * teams * K * N},
-                                x.options().dtype(at::kFloat));
-        const auto op = (ConstOffsets)offsets.data_ptr<int64_t>();
-        hipLaunchKernelGGL((segment_wgrad_wide_kernel<T>), dim3(cus), dim3(512),
-                           0, stream_of_current(), (const T*)xc.data_ptr(),
-                           xc.stride(0), (const T*)gc.data_ptr(), gc.stride(0),
-                           op, (T*)dw.data_ptr(), planes.data_ptr<float>(),
-                           (int)R, (int)G, (int)K, (int)N, (int)wn, (int)wide,
-                           teams);
-        hipLaunchKernelGGL((sum_teams_kernel<T>),
-                           dim3(grid_for(ceil_div(K * N, 4), 256, 1024), G),
-                           dim3(256), 0, stream_of_current(),
-                           planes.data_ptr<float>(), op, (T*)dw.data_ptr(),
-                           (int)R, (int)G, K * N, teams);
+      const int64_t tiles = ceil_div(K, 256) * ceil_div(N, 256);
+      if (whole && K >= 128 && N >= 128 && R >= 512 * G && tiles <= cus) {
+        by_teams(segment_wgrad_wide_kernel<T>, cus, 512, 256, tiles,
+                 (int)(cus / tiles));
         return;
       }
     }
-    auto go = [&](auto* out) {
-      using O = std::remove_pointer_t<decltype(out)>;
-      auto kernel = whole ? segment_mm_wgrad_kernel<T, O, true, B, B, 2, 2>
-                          : segment_mm_wgrad_kernel<T, O, false, B, B, 2, 2>;
-      hipLaunchKernelGGL(kernel, dim3(tiles * splits), dim3(256), 0,
-                         stream_of_current(), (const T*)xc.data_ptr(),
-                         xc.stride(0), (const T*)gc.data_ptr(), gc.stride(0),
-                         (ConstOffsets)offsets.data_ptr<int64_t>(), out, (int)R,
-                         (int)G, (int)K, (int)N, (int)tk, (int)tn, (int)splits);
+    auto pick = [&](auto wv) {
+      constexpr bool W = decltype(wv)::value;
+      constexpr int B = sizeof(T) == 4 ? 64 : 128;
+      const int64_t tk = ceil_div(K, B), tn = ceil_div(N, B), tiles = tk * tn;
+      // fewer blocks than two rounds over the chip: teams of at least 128 rows
+      const int64_t teams =
+          std::min(ceil_div(4 * cus, tiles), ceil_div(R, 128));
+      if (tiles * G < 4 * cus && teams > 1) {
+        by_teams(segment_wgrad_teams_kernel<T, W, B, B, 2, 2>,
+                 (int)(teams * tiles), 256, B, tiles, (int)teams);
+        return;
+      }
+      TORCH_CHECK(tiles * G < INT32_MAX, "segment_mm: too many tiles");
+      hipLaunchKernelGGL((segment_wgrad_kernel<T, W, B, B, 2, 2>),
+                         dim3(tiles * G), dim3(256), 0, stream, xp,
+                         xc.stride(0), gp, gc.stride(0), op, (T*)dw.data_ptr(),
+                         (int)R, (int)K, (int)N, (int)tk, (int)tn);
     };
-    if (splits == 1) {
-      go((T*)dw.data_ptr());
-    } else {
-      auto parts = at::empty({splits * dw.numel()},
-                             x.options().dtype(at::kFloat));
-      go(parts.data_ptr<float>());
-      hipLaunchKernelGGL((sum_parts_kernel<T>),
-                         dim3(grid_for(ceil_div(dw.numel(), 4), 256, 8192)),
-                         dim3(256), 0, stream_of_current(),
-                         parts.data_ptr<float>(), (T*)dw.data_ptr(),
-                         dw.numel(), (int)splits);
-    }
+    whole ? pick(std::true_type{}) : pick(std::false_type{});
   });
   DOA_CHECK_HIP(hipGetLastError());
   return dw;

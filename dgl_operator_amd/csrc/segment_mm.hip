@@ -252,23 +252,23 @@ __device__ inline void store_tile(const f32x4 (&acc)[FM][FN], char* room, O* c,
 }
 
 // two stages of both operands
-constexpr int lds_bytes(int BM, int BN) { return 2 * (BM + BN) * kStepBytes; }
+constexpr int lds_bytes(int BM, int BN, int STEP) { return 2 * (BM + BN) * STEP; }
 
 // c[m][n] = sum_k a(m, k) b(k, n) for one tile of BM x BN. AC, BC: that
 // operand's depth is its outer index. WM x WN waves. WHOLE: every row of both
 // starts on 16 bytes and is whole chunks long.
 template <typename T, typename O, bool AC, bool BC, bool WHOLE, int BM, int BN,
-          int WM, int WN>
+          int WM, int WN, int STEP>
 __device__ inline void tile_product(char* lds, const T* a, int64_t lda, int M,
                                     const T* b, int64_t ldb, int N, int64_t K,
                                     O* c, int64_t ldc) {
   constexpr int THREADS = 64 * WM * WN;
-  using TA = Tile<T, AC, BM, THREADS>;
-  using TB = Tile<T, BC, BN, THREADS>;
+  using TA = Tile<T, AC, BM, THREADS, STEP>;
+  using TB = Tile<T, BC, BN, THREADS, STEP>;
   constexpr int FM = BM / WM / 16, FN = BN / WN / 16;
   constexpr int BK = TA::BK;
   constexpr int STAGE = TA::BYTES + TB::BYTES;
-  static_assert(2 * STAGE == lds_bytes(BM, BN), "LDS");
+  static_assert(2 * STAGE == lds_bytes(BM, BN, STEP), "LDS");
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int wm = wave / WN * (BM / WM), wn = wave % WN * (BN / WN);
   const typename TA::template Reader<FM> read_a(wm);
@@ -277,7 +277,7 @@ __device__ inline void tile_product(char* lds, const T* a, int64_t lda, int M,
   const int64_t step_a = AC ? BK * lda : BK, step_b = BC ? BK * ldb : BK;
   auto multiply = [&](const char* la, const char* lb, int64_t left) {
 #pragma unroll
-    for (int kk = 0; kk < 2; ++kk) {
+    for (int kk = 0; kk < STEP / 64; ++kk) {
       // fp32's matrix rate is worth a branch around zeros
       if (sizeof(T) == 4 && kk && left <= BK / 2) continue;
       typename TA::Frag fa[FM];
@@ -388,18 +388,19 @@ __device__ inline int64_t xcd_order(int64_t b, int64_t blocks) {
   return (b >> 3) < whole ? (b & 7) * whole + (b >> 3) : b;
 }
 
-template <typename T, bool WC, bool WHOLE, int BM, int BN, int WM, int WN>
-__global__ __launch_bounds__(64 * WM * WN, 2) void segment_mm_kernel(
+template <typename T, bool WC, bool WHOLE, int BM, int BN, int WM, int WN,
+          int STEP, int WAVES>
+__global__ __launch_bounds__(64 * WM * WN, WAVES) void segment_mm_kernel(
     const T* __restrict__ x, int64_t xs, const T* __restrict__ w, int64_t wg,
     int64_t wl, ConstOffsets offsets, T* __restrict__ y, int rows, int G, int K,
     int N, int tiles_n) {
   zero_outside(offsets, y, rows, G, N);
   const int work = (int)xcd_order(blockIdx.x, gridDim.x);
-  __shared__ __align__(16) char lds[lds_bytes(BM, BN)];
+  __shared__ __align__(16) char lds[lds_bytes(BM, BN, STEP)];
   const Span s = find_span<BM>(offsets, work / tiles_n, rows, G);
   if (s.many == 0) return;
   const int n0 = work % tiles_n * BN;
-  tile_product<T, T, false, WC, WHOLE, BM, BN, WM, WN>(
+  tile_product<T, T, false, WC, WHOLE, BM, BN, WM, WN, STEP>(
       lds, x + s.r0 * xs, xs, s.many, w + s.g * wg + n0 * (WC ? 1 : wl), wl,
       min(BN, N - n0), K, y + (int64_t)s.r0 * N + n0, N);
 }
@@ -532,6 +533,16 @@ __device__ inline Team team_rows(ConstOffsets offsets, int rows, int G,
   return {first, max(32, ((all + teams - 1) / teams + 31) & ~31)};
 }
 
+// the last group that starts at or before row r
+__device__ inline int group_at(ConstOffsets offsets, int r, int rows, int G) {
+  int lo = 0, hi = G;
+  while (hi - lo > 1) {
+    const int mid = (lo + hi) >> 1;
+    if (offset_at(offsets, mid, rows) <= r) lo = mid; else hi = mid;
+  }
+  return lo;
+}
+
 template <typename T>
 __global__ __launch_bounds__(512) void segment_wgrad_wide_kernel(
     const T* __restrict__ x, int64_t xs, const T* __restrict__ g, int64_t gs,
@@ -557,11 +568,7 @@ __global__ __launch_bounds__(512) void segment_wgrad_wide_kernel(
     while (e < G - 1 && offset_at(offsets, e + 1, rows) <= r) ++e;
     return e;
   };
-  int lo = 0, hi = G;  // the last group that starts at or before `from`
-  while (hi - lo > 1) {
-    const int mid = (lo + hi) >> 1;
-    if (offset_at(offsets, mid, rows) <= from) lo = mid; else hi = mid;
-  }
+  const int lo = group_at(offsets, from, rows, G);
   int use_g = lo, use_r = from, load_g = lo, load_r = from;
   int load_stop = max(from + 1, stop_of(lo));
   uint32_t pa[TT::PER], pb[TT::PER];
@@ -640,11 +647,14 @@ __global__ __launch_bounds__(512) void segment_wgrad_wide_kernel(
   asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
 }
 
-// groups that several teams hold, the teams in order; empty groups
+// Groups that several teams hold, and empty ones. A block has 64 lanes of up to
+// 4 elements; each of its 4 waves sums a quarter of the teams in their order,
+// and the quarters are added in theirs.
 template <typename T>
 __global__ __launch_bounds__(256) void sum_teams_kernel(
     const float* __restrict__ planes, ConstOffsets offsets, T* __restrict__ dw,
     int rows, int G, int64_t n, int teams) {
+  __shared__ f32x4 part[4][64];
   const int e = blockIdx.y;
   const int b = offset_at(offsets, e, rows), s = offset_at(offsets, e + 1, rows);
   const Team tr = team_rows(offsets, rows, G, teams);
@@ -652,63 +662,77 @@ __global__ __launch_bounds__(256) void sum_teams_kernel(
   const int t0 = min(teams - 1, max(0, b - tr.begin) / tr.each);
   const int t1 = min(teams - 1, max(0, s - 1 - tr.begin) / tr.each);
   if (s > b && t0 == t1) return;  // whole in one team
-  for (int64_t i = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 4; i < n;
-       i += (int64_t)gridDim.x * 1024) {
-    if (n % 4 == 0) {
-      f32x4 sum = {};
-      if (s > b)
-        for (int t = t0; t <= t1; ++t)
-          sum += *reinterpret_cast<const f32x4*>(
-              planes + (2 * (int64_t)t + (t == t0)) * n + i);
-      Vec<T, 4> o;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int many = s > b ? t1 - t0 + 1 : 0, each = (many + 3) >> 2;
+  const int from = t0 + min(many, wave * each);
+  const int to = t0 + min(many, wave * each + each);
+  for (int64_t i0 = (int64_t)blockIdx.x * 256; i0 < n;
+       i0 += (int64_t)gridDim.x * 256) {
+    const int64_t i = i0 + lane * 4;
+    const bool whole = n % 4 == 0;  // planes then start on 16 bytes
+    f32x4 sum = {};
+    if (i < n) {
+#pragma unroll 8
+      for (int t = from; t < to; ++t) {
+        const float* p = planes + (2 * (int64_t)t + (t == t0)) * n + i;
+        if (whole) {
+          sum += *reinterpret_cast<const f32x4*>(p);
+        } else {
 #pragma unroll
-      for (int r = 0; r < 4; ++r) o.v[r] = (T)sum[r];
-      *reinterpret_cast<Vec<T, 4>*>(dw + e * n + i) = o;
-    } else {
-      for (int64_t j = i; j < min(n, i + 4); ++j) {
-        float sum = 0.f;
-        if (s > b)
-          for (int t = t0; t <= t1; ++t)
-            sum += planes[(2 * (int64_t)t + (t == t0)) * n + j];
-        dw[e * n + j] = (T)sum;
+          for (int r = 0; r < 4; ++r)
+            if (i + r < n) sum[r] += p[r];
+        }
       }
     }
+    part[wave][lane] = sum;
+    __syncthreads();
+    if (wave == 0 && i < n) {
+      sum = ((part[0][lane] + part[1][lane]) + part[2][lane]) + part[3][lane];
+#pragma unroll
+      for (int r = 0; r < 4; ++r)
+        if (i + r < n) dw[e * n + i + r] = (T)sum[r];
+    }
+    __syncthreads();
   }
 }
 
 // dW by a block for each group and tile: many groups
-template <typename T, bool WHOLE, int BM, int BN, int WM, int WN>
-__global__ __launch_bounds__(64 * WM * WN, 2) void segment_wgrad_kernel(
+template <typename T, bool WHOLE, int BM, int BN, int WM, int WN, int STEP,
+          int WAVES>
+__global__ __launch_bounds__(64 * WM * WN, WAVES) void segment_wgrad_kernel(
     const T* __restrict__ x, int64_t xs, const T* __restrict__ g, int64_t gs,
     ConstOffsets offsets, T* __restrict__ dw, int rows, int K, int N,
     int tiles_k, int tiles_n) {
-  __shared__ __align__(16) char lds[lds_bytes(BM, BN)];
+  __shared__ __align__(16) char lds[lds_bytes(BM, BN, STEP)];
   int work = (int)xcd_order(blockIdx.x, gridDim.x);
   const int n0 = work % tiles_n * BN;
   work /= tiles_n;
   const int k0 = work % tiles_k * BM, e = work / tiles_k;
   const int64_t begin = offset_at(offsets, e, rows);
   const int64_t len = offset_at(offsets, e + 1, rows) - begin;
-  tile_product<T, T, true, true, WHOLE, BM, BN, WM, WN>(
+  tile_product<T, T, true, true, WHOLE, BM, BN, WM, WN, STEP>(
       lds, x + begin * xs + k0, xs, min(BM, K - k0), g + begin * gs + n0, gs,
       min(BN, N - n0), len, dw + ((int64_t)e * K + k0) * N + n0, N);
 }
 
 // dW by teams, as segment_wgrad_wide_kernel: few groups with many rows
-template <typename T, bool WHOLE, int BM, int BN, int WM, int WN>
-__global__ __launch_bounds__(64 * WM * WN, 2) void segment_wgrad_teams_kernel(
+template <typename T, bool WHOLE, int BM, int BN, int WM, int WN, int STEP,
+          int WAVES>
+__global__ __launch_bounds__(64 * WM * WN, WAVES) void segment_wgrad_teams_kernel(
     const T* __restrict__ x, int64_t xs, const T* __restrict__ g, int64_t gs,
     ConstOffsets offsets, T* __restrict__ dw, float* __restrict__ planes,
     int rows, int G, int K, int N, int tiles_n, int tiles, int teams) {
   const int work = (int)xcd_order(blockIdx.x, gridDim.x);
-  __shared__ __align__(16) char lds[lds_bytes(BM, BN)];
+  __shared__ __align__(16) char lds[lds_bytes(BM, BN, STEP)];
   const int team = work / tiles, tile = work % tiles;
   const int k0 = tile / tiles_n * BM, n0 = tile % tiles_n * BN;
   const Team tr = team_rows(offsets, rows, G, teams);
   const int from = tr.begin + (int)min((int64_t)team * tr.each, (int64_t)rows);
   const int to = (int)min((int64_t)from + tr.each,
                           (int64_t)offset_at(offsets, G, rows));
-  for (int r = from, e = 0; r < to;) {
+  if (from >= to) return;
+  int e = group_at(offsets, from, rows, G);
+  for (int r = from; r < to;) {
     while (e < G - 1 && offset_at(offsets, e + 1, rows) <= r) ++e;
     const int g_start = offset_at(offsets, e, rows);
     const int g_stop = offset_at(offsets, e + 1, rows);
@@ -718,11 +742,11 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void segment_wgrad_teams_kernel(
     const int64_t corner = (int64_t)k0 * N + n0;
     __syncthreads();  // the last product's LDS is free
     if (r == g_start && stop == g_stop)
-      tile_product<T, T, true, true, WHOLE, BM, BN, WM, WN>(
+      tile_product<T, T, true, true, WHOLE, BM, BN, WM, WN, STEP>(
           lds, a, xs, min(BM, K - k0), b, gs, min(BN, N - n0), stop - r,
           dw + (int64_t)e * K * N + corner, N);
     else
-      tile_product<T, float, true, true, WHOLE, BM, BN, WM, WN>(
+      tile_product<T, float, true, true, WHOLE, BM, BN, WM, WN, STEP>(
           lds, a, xs, min(BM, K - k0), b, gs, min(BN, N - n0), stop - r,
           planes + (2 * (int64_t)team + (r == g_start)) * K * N + corner, N);
     r = stop;
@@ -824,14 +848,21 @@ at::Tensor segment_mm(at::Tensor offsets, at::Tensor x, at::Tensor weight,
           return;
         }
       }
-      // few rows a group: a tile of 32 rows leaves less of it empty and reads
-      // the weights over more blocks
+      // Few rows a group: a lower tile leaves less of it empty and reads the
+      // weights over more blocks. Above that, steps of 64 bytes let four blocks
+      // share a CU and hide each other's first loads and stores (400 x 400 for
+      // 1345 groups in bf16: 49 rows a group 133 us with 64 rows, 139 with 128;
+      // 195 rows a group 283 and 256, and 277 with steps of 128 bytes).
       if (R <= 48 * G)
-        go(segment_mm_kernel<T, WC, W, 32, 64, 1, 4>, 32, 64, 256);
+        go(segment_mm_kernel<T, WC, W, 32, 64, 1, 4, 128, 2>, 32, 64, 256);
       else if constexpr (sizeof(T) == 4)
-        go(segment_mm_kernel<T, WC, W, 64, 64, 2, 2>, 64, 64, 256);
+        go(segment_mm_kernel<T, WC, W, 64, 64, 2, 2, 128, 2>, 64, 64, 256);
+      else if (R <= 96 * G)
+        go(segment_mm_kernel<T, WC, W, 64, 128, 2, 2, 128, 2>, 64, 128, 256);
+      else if constexpr (W)
+        go(segment_mm_kernel<T, WC, W, 128, 128, 2, 2, 64, 4>, 128, 128, 256);
       else
-        go(segment_mm_kernel<T, WC, W, 128, 128, 2, 2>, 128, 128, 256);
+        go(segment_mm_kernel<T, WC, W, 128, 128, 2, 2, 128, 2>, 128, 128, 256);
     };
     if (wc)
       whole ? pick(std::true_type{}, std::true_type{})
@@ -876,13 +907,15 @@ at::Tensor segment_mm_wgrad(at::Tensor offsets, at::Tensor x, at::Tensor grad) {
                          planes.data_ptr<float>(), (int)R, (int)G, (int)K,
                          (int)N, (int)ceil_div(N, BN), (int)tiles, teams);
       hipLaunchKernelGGL((sum_teams_kernel<T>),
-                         dim3(grid_for(ceil_div(K * N, 4), 256, 1024), G),
+                         dim3(grid_for(K * N, 256, 4096), G),
                          dim3(256), 0, stream, planes.data_ptr<float>(), op,
                          (T*)dw.data_ptr(), (int)R, (int)G, K * N, teams);
     };
     if constexpr (sizeof(T) == 2) {
       const int64_t tiles = ceil_div(K, 256) * ceil_div(N, 256);
-      if (whole && K >= 128 && N >= 128 && R >= 512 * G && tiles <= cus) {
+      // its 256 x 256 tiles want 1024 rows a block to be worth their planes
+      if (whole && K >= 128 && N >= 128 && R >= 512 * G && tiles <= cus &&
+          R / (cus / tiles) >= 1024) {
         by_teams(segment_wgrad_wide_kernel<T>, cus, 512, 256, tiles,
                  (int)(cus / tiles));
         return;
@@ -892,19 +925,34 @@ at::Tensor segment_mm_wgrad(at::Tensor offsets, at::Tensor x, at::Tensor grad) {
       constexpr bool W = decltype(wv)::value;
       constexpr int B = sizeof(T) == 4 ? 64 : 128;
       const int64_t tk = ceil_div(K, B), tn = ceil_div(N, B), tiles = tk * tn;
-      // fewer blocks than two rounds over the chip: teams of at least 128 rows
+      // Where groups and tiles alone are fewer than two blocks a CU: teams, of
+      // rows enough that a team reads as much as its plane costs (8 bytes an
+      // element, written and read).
+      const int64_t each = std::max<int64_t>(256, 2 * K * N / (K + N));
       const int64_t teams =
-          std::min(ceil_div(4 * cus, tiles), ceil_div(R, 128));
-      if (tiles * G < 4 * cus && teams > 1) {
-        by_teams(segment_wgrad_teams_kernel<T, W, B, B, 2, 2>,
+          std::min(ceil_div(2 * cus, tiles), ceil_div(R, each));
+      if (tiles * G < 2 * cus && teams > G) {
+        by_teams(segment_wgrad_teams_kernel<T, W, B, B, 2, 2, 128, 2>,
                  (int)(teams * tiles), 256, B, tiles, (int)teams);
         return;
       }
       TORCH_CHECK(tiles * G < INT32_MAX, "segment_mm: too many tiles");
-      hipLaunchKernelGGL((segment_wgrad_kernel<T, W, B, B, 2, 2>),
-                         dim3(tiles * G), dim3(256), 0, stream, xp,
-                         xc.stride(0), gp, gc.stride(0), op, (T*)dw.data_ptr(),
-                         (int)R, (int)K, (int)N, (int)tk, (int)tn);
+      auto go = [&](auto kernel) {
+        hipLaunchKernelGGL(kernel, dim3(tiles * G), dim3(256), 0, stream, xp,
+                           xc.stride(0), gp, gc.stride(0), op,
+                           (T*)dw.data_ptr(), (int)R, (int)K, (int)N, (int)tk,
+                           (int)tn);
+      };
+      // short groups are a step or two: more blocks a CU hide their ends (400 x
+      // 400 for 1345 groups in bf16, 49 rows a group: 174 us, and 233 with steps
+      // of 128 bytes; 437 rows a group of 256 x 512: 223 and 185)
+      if constexpr (W && sizeof(T) == 2) {
+        if (R <= 256 * G) {
+          go(segment_wgrad_kernel<T, W, B, B, 2, 2, 64, 4>);
+          return;
+        }
+      }
+      go(segment_wgrad_kernel<T, W, B, B, 2, 2, 128, 2>);
     };
     whole ? pick(std::true_type{}) : pick(std::false_type{});
   });

@@ -16,6 +16,8 @@ namespace doa {
 
 constexpr int kTopMost = 32;
 
+using f32x4 = __attribute__((__vector_size__(4 * sizeof(float)))) float;
+
 // larger key = earlier alternative; 0 is below every element's key
 __device__ inline uint64_t top_key(float z, int j) {
   // -0 and +0 are equal values; every NaN is the largest
@@ -80,6 +82,10 @@ template <>
 struct SmallKey<float> {
   using type = uint64_t;
   static __device__ uint64_t make(float z, int j) { return top_key(z, j); }
+  static __device__ uint64_t quick(float z, int j) {  // not for NaN
+    const int32_t b = (int32_t)__float_as_uint(z + 0.f);
+    return (uint64_t)(uint32_t)(b ^ (b >> 31 | INT32_MIN)) << 32 | (uint32_t)~j;
+  }
   static __device__ int index(uint64_t k) { return key_index(k); }
   static __device__ float value(uint64_t k) { return key_value(k); }
   // x into the falling list; the last one drops out
@@ -103,6 +109,13 @@ struct SmallKey {  // 16-bit types: the index has 16 bits too
     if (v != v) b = 0x7fffu;
     b = (b & 0x8000u) ? ~b & 0xffffu : b | 0x8000u;
     return b << 16 | (0xffffu - j);
+  }
+  static __device__ uint32_t quick(T v, int j) {  // not for NaN
+    // -0 + 0 is +0; the sign turns the order of the negative round
+    const int32_t b =
+        (int32_t)__builtin_bit_cast(uint16_t, (T)(v + (T)0.f)) << 16;
+    const uint32_t o = b ^ (b >> 31 | INT32_MIN);
+    return (o & 0xffff0000u) | (0xffffu - j);
   }
   static __device__ int index(uint32_t k) { return 0xffff - (k & 0xffffu); }
   static __device__ float value(uint32_t k) {
@@ -158,35 +171,46 @@ __global__ __launch_bounds__(256) void log_probs_short_kernel(
   const int r = lane / L, part = lane % L;
   const bool live = r < many;
   const T* zr = tile + (live ? r : 0) * C;
-  // my elements: part, part + L, ... begun at a place of my own
+  // my elements: part, part + L, ... begun at a place of my own where rows of
+  // even length would start on the same banks
   const int count = (C - part + L - 1) / L;
-  int begin = (C & 1) || count < 1 ? 0 : r % count;
-  typename Key::type best[K > 0 ? K : 1];
+  const int begin = (C & 1) || count < 1 ? 0 : r % count;
+  // (element by element: wider reads would straddle the rows' odd alignment)
+  using Bits = std::conditional_t<sizeof(T) == 4, uint32_t, uint16_t>;
+  const auto* zb =
+      (const volatile __attribute__((address_space(3))) Bits*)zr;
+  auto at = [&](int j) { return __builtin_bit_cast(T, (Bits)zb[j]); };
+  auto walk = [&](auto visit) {
+    if (C & 1) {
+#pragma unroll 4
+      for (int i = 0; i < count; ++i) visit(at(i * L + part), i * L + part);
+    } else {
+#pragma unroll 4
+      for (int i = begin; i < count; ++i) visit(at(i * L + part), i * L + part);
+#pragma unroll 4
+      for (int i = 0; i < begin; ++i) visit(at(i * L + part), i * L + part);
+    }
+  };
+  constexpr int S = K > 0 ? K : 1;
+  typename Key::type best[S];
+  auto find_best = [&](auto make) {
 #pragma unroll
-  for (int i = 0; i < (K > 0 ? K : 1); ++i) best[i] = 0;
-  float m = -INFINITY;
-  for (int i = 0, at = begin; i < count; ++i) {
-    const int j = at * L + part;
-    const T v = zr[j];
-    if constexpr (K > 0) Key::template insert<K>(best, Key::make(v, j));
-    else m = fmaxf(m, (float)v);
-    if (++at == count) at = 0;
-  }
-  if constexpr (K > 0) {
+    for (int i = 0; i < S; ++i) best[i] = 0;
+    walk([&](T v, int j) { Key::template insert<S>(best, make(v, j)); });
 #pragma unroll
     for (int d = 1; d < L; d <<= 1) {
-      typename Key::type other[K];
+      typename Key::type other[S];
 #pragma unroll
-      for (int i = 0; i < K; ++i) other[i] = shuffle_key(best[i], d);
-      if constexpr ((K & (K - 1)) == 0) {
+      for (int i = 0; i < S; ++i) other[i] = shuffle_key(best[i], d);
+      if constexpr ((S & (S - 1)) == 0) {
         // one list against the other turned round leaves the K best, first
         // rising then falling: log K exchanges sort them
 #pragma unroll
-        for (int i = 0; i < K; ++i) best[i] = max(best[i], other[K - 1 - i]);
+        for (int i = 0; i < S; ++i) best[i] = max(best[i], other[S - 1 - i]);
 #pragma unroll
-        for (int h = K / 2; h > 0; h /= 2)
+        for (int h = S / 2; h > 0; h /= 2)
 #pragma unroll
-          for (int i = 0; i < K; ++i)
+          for (int i = 0; i < S; ++i)
             if (!(i & h)) {
               const auto x = best[i], y = best[i + h];
               best[i] = max(x, y);
@@ -194,24 +218,33 @@ __global__ __launch_bounds__(256) void log_probs_short_kernel(
             }
       } else {
 #pragma unroll
-        for (int i = 0; i < K; ++i) Key::template insert<K>(best, other[i]);
+        for (int i = 0; i < S; ++i) Key::template insert<S>(best, other[i]);
       }
     }
+  };
+  float m = -INFINITY;
+  if constexpr (K > 0) {
+    find_best([](T v, int j) { return Key::quick(v, j); });
     m = Key::value(best[0]);
   } else {
+    walk([&](T v, int) { m = fmaxf(m, (float)v); });
 #pragma unroll
     for (int d = 1; d < L; d <<= 1) m = fmaxf(m, __shfl_xor(m, d));
   }
   const float base = m == -INFINITY ? 0.f : m;
   float s = 0.f, a = 0.f;
-  for (int i = 0, at = begin; i < count; ++i) {
-    add_term((float)zr[at * L + part], base, s, a);
-    if (++at == count) at = 0;
-  }
+  walk([&](T v, int) { add_term((float)v, base, s, a); });
 #pragma unroll
   for (int d = 1; d < L; d <<= 1) {
     s += __shfl_xor(s, d);
     a += __shfl_xor(a, d);
+  }
+  if constexpr (K > 0) {
+    // a NaN has spoiled its row's sum and may have lost its place
+    if (__ballot(s != s)) {
+      find_best([](T v, int j) { return Key::make(v, j); });
+      m = Key::value(best[0]);
+    }
   }
   if (!live || part != 0) return;
   const int64_t row = row0 + r;
@@ -251,16 +284,16 @@ struct LongShared {
 };
 
 // the k largest of the block's keys, falling, each given to emit(rank, key)
-template <int NT, typename Emit>
-__device__ inline void best_of_block(const float (&v)[kPer], int first, int c1,
-                                     const int (&index)[kPer], int k,
-                                     LongShared<NT>& sh, Emit emit) {
+template <int NT, int E, typename Emit>
+__device__ inline void best_of_block(const float (&v)[kPer], int c0, int c1,
+                                     int k, LongShared<NT>& sh, Emit emit) {
   const float t = sh.threshold;
+  auto index = [&](int i) { return c0 + ((i / E) * NT + (int)threadIdx.x) * E + i % E; };
 #pragma unroll
   for (int i = 0; i < kPer; ++i)
-    if (!(v[i] < t) && index[i] < c1) {
+    if (!(v[i] < t) && index(i) < c1) {
       const int at = atomicAdd(&sh.count, 1);
-      if (at < kCap) sh.keys[at] = top_key(v[i], index[i]);
+      if (at < kCap) sh.keys[at] = top_key(v[i], index(i));
     }
   __syncthreads();
   const int count = sh.count;
@@ -276,12 +309,17 @@ __device__ inline void best_of_block(const float (&v)[kPer], int first, int c1,
     return;
   }
   uint64_t last = ~0ull;
+#pragma unroll 1
   for (int r = 0; r < k; ++r) {
     uint64_t best = 0;
+    // (the keys are made again each time: kept, they would cost every block
+    // the registers of a second one on the CU)
 #pragma unroll
     for (int i = 0; i < kPer; ++i)
-      if (index[i] < c1) {
-        const uint64_t key = top_key(v[i], index[i]);
+      if (index(i) < c1) {
+        float z = v[i];
+        asm volatile("" : "+v"(z));
+        const uint64_t key = top_key(z, index(i));
         if (key < last && key > best) best = key;
       }
 #pragma unroll
@@ -301,7 +339,7 @@ __device__ inline void best_of_block(const float (&v)[kPer], int first, int c1,
 // the value that k of a wave's 64 values reach (-inf: fewer than k are above)
 __device__ inline float kth_of_wave(float v, int k) {
   int reach = 0;
-#pragma unroll
+#pragma unroll 8
   for (int i = 0; i < 64; ++i) {
     const float o = __uint_as_float(
         __builtin_amdgcn_readlane(__float_as_uint(v), i));
@@ -329,7 +367,6 @@ __global__ __launch_bounds__(NT) void log_probs_long_kernel(
   const T* zr = z + row * zs;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   float v[kPer];
-  int index[kPer];
   float m = -INFINITY;
 #pragma unroll
   for (int i = 0; i < kPer / E; ++i) {
@@ -345,7 +382,6 @@ __global__ __launch_bounds__(NT) void log_probs_long_kernel(
 #pragma unroll
     for (int e = 0; e < E; ++e) {
       v[i * E + e] = (float)u.e[e];
-      index[i * E + e] = j + e;
       m = fmaxf(m, v[i * E + e]);
     }
   }
@@ -388,7 +424,7 @@ __global__ __launch_bounds__(NT) void log_probs_long_kernel(
       o[2] = a;
     }
     if (k > 0)
-      best_of_block<NT>(v, c0, c1, index, k, sh, [&](int r, uint64_t key) {
+      best_of_block<NT, E>(v, c0, c1, k, sh, [&](int r, uint64_t key) {
         part_keys[(int64_t)blockIdx.x * k + r] = key;
       });
     return;
@@ -399,7 +435,7 @@ __global__ __launch_bounds__(NT) void log_probs_long_kernel(
     if (target) write_answer(zr, st, row, target, ignore, C, lp);
   }
   if (k > 0)
-    best_of_block<NT>(v, c0, c1, index, k, sh, [&](int r, uint64_t key) {
+    best_of_block<NT, E>(v, c0, c1, k, sh, [&](int r, uint64_t key) {
       top_idx[row * k + r] = key_index(key);
       top_lp[row * k + r] = st.log_p(key_value(key));
     });
@@ -508,78 +544,100 @@ __global__ __launch_bounds__(256) void log_probs_bwd_kernel(
     int tile_rows, int col_tiles, uint64_t magic, T* __restrict__ dz) {
   __shared__ __align__(16) float tile[kTileElems];
   __shared__ RowPull info[kTileRows];
-  constexpr int E = 16 / sizeof(T);
+  __shared__ float own[kTileRows * kTopMost];
+  constexpr int E = 16 / sizeof(T), PER = kTileElems / (256 * E);
   const int64_t row0 = blockIdx.x / col_tiles * (int64_t)tile_rows;
   const int c0 = blockIdx.x % col_tiles * kTileElems;
   const int many = (int)min((int64_t)tile_rows, rows - row0);
   const int W = min(kTileElems, C - c0);  // = C where a tile has many rows
   const int n = many * W;
+  // all loads first: what the tile needs and the logits themselves
+  const T* src = z + row0 * zs + c0;
+  const bool flat = zs == W || many == 1;
+  union Part { Chunk q; T e[E]; };
+  Part part[PER];
+#pragma unroll
+  for (int p = 0; p < PER; ++p) {
+    const int i = (p * 256 + threadIdx.x) * E;
+    if (flat && i + E <= n) {
+      part[p].q = *reinterpret_cast<const LooseChunk*>(src + i);
+    } else if (i < n) {
+      // i / W by a product: exact for i below 2^12
+      int r = (int)((i * magic) >> 32), c = i - r * W;
+#pragma unroll
+      for (int e = 0; e < E; ++e) {
+        part[p].e[e] = i + e < n ? src[r * zs + c] : (T)0.f;
+        if (++c == W) c = 0, ++r;
+      }
+    }
+  }
+  const int tops = g_top ? many * k : 0;
+  for (int i = threadIdx.x; i < tops; i += 256) own[i] = g_top[row0 * k + i];
+  int64_t t = -1;
+  float gl = 0.f;
+  RowPull p{};
   if (threadIdx.x < many) {
     const int64_t row = row0 + threadIdx.x;
-    RowPull p;
-    p.base = stats[2 * row];
-    p.logs = stats[2 * row + 1];
-    p.pull = 0.f;
+    p = {stats[2 * row], stats[2 * row + 1], 0.f, g_ent ? g_ent[row] : 0.f,
+         ent[row]};
     if (target && g_lp) {
-      const int64_t t = target[row];
-      p.pull = t == ignore ? 0.f : (t >= 0 && t < C) ? g_lp[row] : NAN;
+      t = target[row];
+      gl = t == ignore ? 0.f : (t >= 0 && t < C) ? g_lp[row] : NAN;
     }
+  }
+  const int first_top =
+      threadIdx.x < tops ? (int)(top_idx[row0 * k + threadIdx.x] - c0) : -1;
+  __syncthreads();
+  if (threadIdx.x < many) {
+    p.pull = gl;
     if (g_top)
-      for (int i = 0; i < k; ++i) p.pull += g_top[row * k + i];
-    p.gh = g_ent ? g_ent[row] : 0.f;
-    p.ent = ent[row];
+      for (int i = 0; i < k; ++i) p.pull += own[threadIdx.x * k + i];
     info[threadIdx.x] = p;
   }
   __syncthreads();
-  const T* src = z + row0 * zs + c0;
-  const bool flat = zs == W || many == 1;
-  for (int i = threadIdx.x * E; i < n; i += 256 * E) {
-    // i / W by a product: exact for i below 2^12
-    int r = (int)((i * magic) >> 32), c = i - r * W;
-    union { Chunk q; T e[E]; } u;
-    if (flat && i + E <= n) {
-      u.q = *reinterpret_cast<const LooseChunk*>(src + i);
-    } else {
-      int rr = r, cc = c;
 #pragma unroll
-      for (int e = 0; e < E; ++e) {
-        if (i + e < n) u.e[e] = src[rr * zs + cc];
-        if (++cc == W) cc = 0, ++rr;
-      }
-    }
+  for (int q = 0; q < PER; ++q) {
+    const int i = (q * 256 + threadIdx.x) * E;
+    if (i >= n) break;
+    int r = (int)((i * magic) >> 32), c = i - r * W;
+    union { f32x4 v[E / 4]; float e[E]; } g;
 #pragma unroll
     for (int e = 0; e < E; ++e) {
-      if (i + e < n) {
-        const RowPull& p = info[r];
-        const float l = ((float)u.e[e] - p.base) - p.logs;
-        const float g =
-            -__expf(l) * (p.pull + p.gh * (fmaxf(l, -1e30f) + p.ent));
-        tile[i + e] = p.logs == INFINITY ? 0.f : g;
-      }
-      if (++c == W) c = 0, ++r;
+      const RowPull& u = info[r];
+      const float l = ((float)part[q].e[e] - u.base) - u.logs;
+      const float v = -__expf(l) * (u.pull + u.gh * (fmaxf(l, -1e30f) + u.ent));
+      g.e[e] = u.logs == INFINITY ? 0.f : v;
+      // (behind the last row: any row there is)
+      if (++c == W) c = 0, r = min(r + 1, many - 1);
     }
+#pragma unroll
+    for (int e = 0; e < E / 4; ++e)
+      *reinterpret_cast<f32x4*>(tile + i + 4 * e) = g.v[e];
   }
   __syncthreads();
-  if (g_top)
-    for (int i = threadIdx.x; i < many * k; i += 256) {
-      const int r = i / k;
-      const int64_t j = top_idx[row0 * k + i] - c0;
-      if (j >= 0 && j < W && info[r].logs != INFINITY)
-        tile[r * W + j] += g_top[row0 * k + i];
-    }
-  __syncthreads();
-  if (target && g_lp && threadIdx.x < many) {
-    const int64_t t = target[row0 + threadIdx.x];
-    if (t != ignore && t >= c0 && t < c0 + W && info[threadIdx.x].logs != INFINITY)
-      tile[threadIdx.x * W + (t - c0)] += g_lp[row0 + threadIdx.x];
+  for (int i = threadIdx.x; i < tops; i += 256) {
+    const int r = i / k;
+    const int j = i == (int)threadIdx.x ? first_top
+                                        : (int)(top_idx[row0 * k + i] - c0);
+    if (j >= 0 && j < W && info[r].logs != INFINITY) tile[r * W + j] += own[i];
   }
+  __syncthreads();
+  if (threadIdx.x < many && t >= c0 && t < c0 + W && t != ignore &&
+      p.logs != INFINITY)
+    tile[threadIdx.x * W + (int)(t - c0)] += gl;
   __syncthreads();
   T* out = dz + row0 * C + c0;  // rows of a tile follow each other
-  for (int i = threadIdx.x * E; i < n; i += 256 * E) {
-    union { Chunk q; T e[E]; } u;
 #pragma unroll
-    for (int e = 0; e < E; ++e)
-      u.e[e] = i + e < n ? (T)tile[i + e] : (T)0.f;
+  for (int q = 0; q < PER; ++q) {
+    const int i = (q * 256 + threadIdx.x) * E;
+    if (i >= n) break;
+    union { f32x4 v[E / 4]; float e[E]; } g;
+#pragma unroll
+    for (int e = 0; e < E / 4; ++e)
+      g.v[e] = *reinterpret_cast<const f32x4*>(tile + i + 4 * e);
+    Part u;
+#pragma unroll
+    for (int e = 0; e < E; ++e) u.e[e] = (T)g.e[e];
     if (i + E <= n) {
       *reinterpret_cast<LooseChunk*>(out + i) = u.q;
     } else {

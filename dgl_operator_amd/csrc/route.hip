@@ -57,29 +57,34 @@ __device__ inline int block_exclusive(int v, int* sums, int* total) {
 }
 
 // one wave puts its slots [lo, hi) in order, from where `next` says the next
-// slot of each group goes
+// slot of each group goes; 4 x 64 ids are on their way at once
 template <typename IdT>
 __device__ inline void place_tile(const IdT* ids, int64_t lo, int64_t hi,
                                   int G, int bits, int* next,
                                   int* __restrict__ position,
                                   int* __restrict__ source) {
   const int lane = threadIdx.x & 63;
-  for (int64_t base = lo; base < hi; base += 64) {
-    const int64_t f = base + lane;
-    const int id = load_id(ids, f, hi, G);
-    const bool valid = id >= 0;
-    const uint64_t same = same_id_lanes(id, valid, bits);
-    int p = -1;
-    if (valid) {
-      const uint64_t below = same & ((1ull << lane) - 1);
-      p = next[id] + __popcll(below);
-      // the last of the lanes moves the group's counter on (a wave's LDS
-      // operations keep their order)
-      if ((same >> lane) == 1ull) next[id] = p + 1;
-      source[p] = (int)f;
+  for (int64_t base = lo; base < hi; base += 256) {
+    int id[4];
+#pragma unroll
+    for (int u = 0; u < 4; ++u) id[u] = load_id(ids, base + u * 64 + lane, hi, G);
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      const int64_t f = base + u * 64 + lane;
+      const bool valid = id[u] >= 0;
+      const uint64_t same = same_id_lanes(id[u], valid, bits);
+      int p = -1;
+      if (valid) {
+        const uint64_t below = same & ((1ull << lane) - 1);
+        p = next[id[u]] + __popcll(below);
+        // the last of the lanes moves the group's counter on (a wave's LDS
+        // operations keep their order)
+        if ((same >> lane) == 1ull) next[id[u]] = p + 1;
+        source[p] = (int)f;
+      }
+      wave_sync();
+      if (f < hi) position[f] = p;
     }
-    wave_sync();
-    if (f < hi) position[f] = p;
   }
 }
 
@@ -126,25 +131,22 @@ __global__ __launch_bounds__(1024) void route_small_kernel(
   for (int p = carry + threadIdx.x; p < n; p += blockDim.x) source[p] = -1;
 }
 
-// ---- many slots: count, scan over tiles, place -----------------------------
+// ---- many slots: count, scan over tiles, place; a wave a tile --------------
 template <typename IdT>
-__global__ __launch_bounds__(256) void route_count_kernel(
+__global__ __launch_bounds__(64) void route_count_kernel(
     const IdT* __restrict__ ids, int64_t n, int G, int tile, int tiles,
     int* __restrict__ counts) {  // [G][tiles]
   extern __shared__ int hist[];
-  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
-  const int t = blockIdx.x * (blockDim.x >> 6) + wave;
-  int* mine = hist + wave * G;
-  for (int g = lane; g < G; g += 64) mine[g] = 0;
+  const int lane = threadIdx.x, t = blockIdx.x;
+  for (int g = lane; g < G; g += 64) hist[g] = 0;
   wave_sync();
-  if (t >= tiles) return;
   const int64_t lo = (int64_t)t * tile, hi = min(n, lo + tile);
   for (int64_t f = lo + lane; f < hi; f += 64) {
     const int id = load_id(ids, f, n, G);
-    if (id >= 0) atomicAdd(&mine[id], 1);
+    if (id >= 0) atomicAdd(&hist[id], 1);
   }
   wave_sync();
-  for (int g = lane; g < G; g += 64) counts[(int64_t)g * tiles + t] = mine[g];
+  for (int g = lane; g < G; g += 64) counts[(int64_t)g * tiles + t] = hist[g];
 }
 
 // each block: one group's counts over the tiles, to exclusive sums
@@ -165,40 +167,39 @@ __global__ __launch_bounds__(256) void route_scan_kernel(
 }
 
 template <typename IdT>
-__global__ __launch_bounds__(256) void route_place_kernel(
+__global__ __launch_bounds__(64) void route_place_kernel(
     const IdT* __restrict__ ids, int64_t n, int G, int bits, int tile,
     int tiles, const int* __restrict__ counts, const int* __restrict__ totals,
     int64_t* __restrict__ offsets, int* __restrict__ position,
     int* __restrict__ source) {
-  extern __shared__ int next[];  // [waves][G]
-  __shared__ int sums[4];
-  const int wave = threadIdx.x >> 6;
-  const int waves = blockDim.x >> 6;
-  const int first = blockIdx.x * waves;
-  // every block sums up the groups' totals by itself
+  extern __shared__ int next[];
+  const int lane = threadIdx.x, t = blockIdx.x;
+  // every wave sums up the groups' totals by itself: less than a launch
   int carry = 0;
-  for (int base = 0; base < G; base += blockDim.x) {
-    const int g = base + threadIdx.x;
+#pragma unroll 4
+  for (int base = 0; base < G; base += 64) {
+    const int g = base + lane;
     const int v = g < G ? totals[g] : 0;
-    int all;
-    const int at = carry + block_exclusive(v, sums, &all);
-    carry += all;
-    if (g < G) {
-      if (blockIdx.x == 0) offsets[g] = at;
-      for (int w = 0; w < waves; ++w)
-        if (first + w < tiles)
-          next[w * G + g] = at + counts[(int64_t)g * tiles + first + w];
+    const int before = g < G ? counts[(int64_t)g * tiles + t] : 0;
+    int inc = v;
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) {
+      const int o = __shfl_up(inc, d);
+      if (lane >= d) inc += o;
     }
+    const int at = carry + inc - v;
+    if (g < G) {
+      next[g] = at + before;
+      if (t == 0) offsets[g] = at;
+    }
+    carry += __shfl(inc, 63);
   }
-  if (blockIdx.x == 0 && threadIdx.x == 0) offsets[G] = carry;
-  __syncthreads();
-  const int t = first + wave;
-  if (t < tiles) {
-    const int64_t lo = (int64_t)t * tile, hi = min(n, lo + tile);
-    place_tile(ids, lo, hi, G, bits, next + wave * G, position, source);
-  }
-  for (int64_t p = carry + (int64_t)blockIdx.x * blockDim.x + threadIdx.x;
-       p < n; p += (int64_t)gridDim.x * blockDim.x)
+  if (t == 0 && lane == 0) offsets[G] = carry;
+  wave_sync();
+  const int64_t lo = (int64_t)t * tile, hi = min(n, lo + tile);
+  place_tile(ids, lo, hi, G, bits, next, position, source);
+  for (int64_t p = carry + (int64_t)t * 64 + lane; p < n;
+       p += (int64_t)tiles * 64)
     source[p] = -1;
 }
 
@@ -236,26 +237,23 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor> route_rows(at::Tensor ids,
       return;
     }
     // a tile's G counters are written and read once more: a tile of G/4 slots
-    // keeps them at a few bytes a slot; at least 512 slots a wave, and no more
-    // tiles than fill the chip
+    // keeps them at a few bytes a slot; at least 256 slots, and no more tiles
+    // than fill the chip
     const int64_t want =
-        std::max<int64_t>({512, G / 4, ceil_div(n, 8192)});
+        std::max<int64_t>({256, G / 4, ceil_div(n, 8192)});
     const int tile = (int)ceil_div(want, 64) * 64;
     const int tiles = (int)ceil_div(n, tile);
-    const int waves = std::min(4, fit);
-    auto counts = at::empty({(int64_t)G * tiles}, i32);
-    auto totals = at::empty({G}, i32);
-    const int blocks = (int)ceil_div(tiles, waves);
-    const size_t lds = (size_t)waves * G * sizeof(int);
-    hipLaunchKernelGGL((route_count_kernel<IdT>), dim3(blocks),
-                       dim3(64 * waves), lds, stream, idp, n, G, tile, tiles,
-                       counts.data_ptr<int>());
+    auto counts = at::empty({(int64_t)G * tiles + G}, i32);
+    int* cp = counts.data_ptr<int>();
+    int* totals = cp + (int64_t)G * tiles;
+    const size_t lds = (size_t)G * sizeof(int);
+    hipLaunchKernelGGL((route_count_kernel<IdT>), dim3(tiles), dim3(64), lds,
+                       stream, idp, n, G, tile, tiles, cp);
     hipLaunchKernelGGL(route_scan_kernel, dim3(G),
-                       dim3(tiles <= 64 ? 64 : 256), 0, stream,
-                       counts.data_ptr<int>(), tiles, totals.data_ptr<int>());
-    hipLaunchKernelGGL((route_place_kernel<IdT>), dim3(blocks),
-                       dim3(64 * waves), lds, stream, idp, n, G, bits, tile,
-                       tiles, counts.data_ptr<int>(), totals.data_ptr<int>(),
+                       dim3(tiles <= 64 ? 64 : 256), 0, stream, cp, tiles,
+                       totals);
+    hipLaunchKernelGGL((route_place_kernel<IdT>), dim3(tiles), dim3(64), lds,
+                       stream, idp, n, G, bits, tile, tiles, cp, totals,
                        offsets.data_ptr<int64_t>(), position.data_ptr<int>(),
                        source.data_ptr<int>());
   };

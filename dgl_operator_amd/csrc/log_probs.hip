@@ -262,7 +262,7 @@ __global__ __launch_bounds__(256) void log_probs_short_kernel(
 }
 
 // ---------------------------------------------------------------------------
-// Long rows: a block holds up to 16 logits a thread in registers and reads
+// Long rows: a block holds a row's logits in registers, PER a thread, and reads
 // them once; rows longer than that are split over blocks and joined.
 //
 // The best k: the 64 lanes' maxima (over the block's waves) give a threshold,
@@ -270,7 +270,6 @@ __global__ __launch_bounds__(256) void log_probs_short_kernel(
 // collected (about k of them) and ranked by counting. Where ties or masks let
 // too many through, k rounds of a block maximum find them one by one.
 // ---------------------------------------------------------------------------
-constexpr int kPer = 16;    // logits a thread
 constexpr int kCap = 512;   // collected candidates
 
 template <int NT>
@@ -283,18 +282,40 @@ struct LongShared {
   int count;
 };
 
-// the k largest of the block's keys, falling, each given to emit(rank, key)
-template <int NT, int E, typename Emit>
-__device__ inline void best_of_block(const float (&v)[kPer], int c0, int c1,
-                                     int k, LongShared<NT>& sh, Emit emit) {
-  const float t = sh.threshold;
-  auto index = [&](int i) { return c0 + ((i / E) * NT + (int)threadIdx.x) * E + i % E; };
+// a thread's part of a row as it was read
+template <typename T, int PER>
+struct Logits {
+  static constexpr int E = 16 / sizeof(T);
+  union Part { Chunk q; T e[E]; };
+  Part part[PER / E];
+  __device__ float at(int i, int e) const { return (float)part[i].e[e]; }
+  // what was made of the logits is made again when it is wanted: kept, it would
+  // cost the registers of the other blocks on the CU
+  __device__ void anew() {
 #pragma unroll
-  for (int i = 0; i < kPer; ++i)
-    if (!(v[i] < t) && index(i) < c1) {
-      const int at = atomicAdd(&sh.count, 1);
-      if (at < kCap) sh.keys[at] = top_key(v[i], index(i));
-    }
+    for (int i = 0; i < PER / E; ++i) asm volatile("" : "+v"(part[i].q));
+  }
+};
+
+// the k largest of the block's keys, falling, each given to emit(rank, key)
+template <typename T, int NT, int PER, typename Emit>
+__device__ inline void best_of_block(Logits<T, PER>& v, const T* zr, int c0,
+                                     int c1, int k, LongShared<NT>& sh,
+                                     Emit emit) {
+  constexpr int E = Logits<T, PER>::E;
+  const float t = sh.threshold;
+  v.anew();
+#pragma unroll
+  for (int i = 0; i < PER / E; ++i) {
+    const int j = c0 + (i * NT + (int)threadIdx.x) * E;
+#pragma unroll
+    for (int e = 0; e < E; ++e)
+      if (!(v.at(i, e) < t) && j + e < c1) {
+        const int at = atomicAdd(&sh.count, 1);
+        if (at < kCap) sh.keys[at] = top_key(v.at(i, e), j + e);
+      }
+    __builtin_amdgcn_sched_barrier(0);
+  }
   __syncthreads();
   const int count = sh.count;
   if (count <= kCap) {
@@ -309,19 +330,13 @@ __device__ inline void best_of_block(const float (&v)[kPer], int c0, int c1,
     return;
   }
   uint64_t last = ~0ull;
-#pragma unroll 1
   for (int r = 0; r < k; ++r) {
     uint64_t best = 0;
-    // (the keys are made again each time: kept, they would cost every block
-    // the registers of a second one on the CU)
-#pragma unroll
-    for (int i = 0; i < kPer; ++i)
-      if (index(i) < c1) {
-        float z = v[i];
-        asm volatile("" : "+v"(z));
-        const uint64_t key = top_key(z, index(i));
-        if (key < last && key > best) best = key;
-      }
+    // (from memory again: rare, and registers would cost a block on the CU)
+    for (int j = c0 + threadIdx.x; j < c1; j += NT) {
+      const uint64_t key = top_key((float)zr[j], j);
+      if (key < last && key > best) best = key;
+    }
 #pragma unroll
     for (int d = 1; d < 64; d <<= 1) {
       const uint64_t o = shuffle_key(best, d);
@@ -351,8 +366,9 @@ __device__ inline float kth_of_wave(float v, int k) {
   return t;
 }
 
-template <typename T, int NT>
-__global__ __launch_bounds__(NT) void log_probs_long_kernel(
+// (64 registers: two blocks of 1024 threads a CU)
+template <typename T, int NT, int PER>
+__global__ __launch_bounds__(NT, 8) void log_probs_long_kernel(
     const T* __restrict__ z, int64_t zs, const int64_t* __restrict__ target,
     int64_t ignore, int C, int k, int splits, int chunk,
     float* __restrict__ lp, float* __restrict__ ent,
@@ -366,25 +382,23 @@ __global__ __launch_bounds__(NT) void log_probs_long_kernel(
   const int c0 = part * chunk, c1 = min(C, c0 + chunk);
   const T* zr = z + row * zs;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  float v[kPer];
+  Logits<T, PER> v;
   float m = -INFINITY;
 #pragma unroll
-  for (int i = 0; i < kPer / E; ++i) {
+  for (int i = 0; i < PER / E; ++i) {
     const int j = c0 + (i * NT + threadIdx.x) * E;
-    union { Chunk q; T e[E]; } u;
     if (j + E <= c1) {
-      u.q = *reinterpret_cast<const LooseChunk*>(zr + j);
+      v.part[i].q = *reinterpret_cast<const LooseChunk*>(zr + j);
     } else {
 #pragma unroll
       for (int e = 0; e < E; ++e)
-        u.e[e] = j + e < c1 ? zr[j + e] : (T)-INFINITY;
-    }
-#pragma unroll
-    for (int e = 0; e < E; ++e) {
-      v[i * E + e] = (float)u.e[e];
-      m = fmaxf(m, v[i * E + e]);
+        v.part[i].e[e] = j + e < c1 ? zr[j + e] : (T)-INFINITY;
     }
   }
+#pragma unroll
+  for (int i = 0; i < PER / E; ++i)
+#pragma unroll
+    for (int e = 0; e < E; ++e) m = fmaxf(m, v.at(i, e));
   sh.lane_max[wave][lane] = m;
   if (threadIdx.x == 0) sh.count = 0;
   __syncthreads();
@@ -398,8 +412,13 @@ __global__ __launch_bounds__(NT) void log_probs_long_kernel(
   for (int d = 1; d < 64; d <<= 1) m = fmaxf(m, __shfl_xor(m, d));
   const float base = m == -INFINITY ? 0.f : m;
   float s = 0.f, a = 0.f;
+  v.anew();
 #pragma unroll
-  for (int i = 0; i < kPer; ++i) add_term(v[i], base, s, a);
+  for (int i = 0; i < PER / E; ++i) {
+#pragma unroll
+    for (int e = 0; e < E; ++e) add_term(v.at(i, e), base, s, a);
+    __builtin_amdgcn_sched_barrier(0);  // not all exponentials at once
+  }
 #pragma unroll
   for (int d = 1; d < 64; d <<= 1) {
     s += __shfl_xor(s, d);
@@ -424,7 +443,7 @@ __global__ __launch_bounds__(NT) void log_probs_long_kernel(
       o[2] = a;
     }
     if (k > 0)
-      best_of_block<NT, E>(v, c0, c1, k, sh, [&](int r, uint64_t key) {
+      best_of_block<T, NT, PER>(v, zr, c0, c1, k, sh, [&](int r, uint64_t key) {
         part_keys[(int64_t)blockIdx.x * k + r] = key;
       });
     return;
@@ -435,7 +454,7 @@ __global__ __launch_bounds__(NT) void log_probs_long_kernel(
     if (target) write_answer(zr, st, row, target, ignore, C, lp);
   }
   if (k > 0)
-    best_of_block<NT, E>(v, c0, c1, k, sh, [&](int r, uint64_t key) {
+    best_of_block<T, NT, PER>(v, zr, c0, c1, k, sh, [&](int r, uint64_t key) {
       top_idx[row * k + r] = key_index(key);
       top_lp[row * k + r] = st.log_p(key_value(key));
     });
@@ -714,8 +733,9 @@ log_probs_fwd(at::Tensor logits, c10::optional<at::Tensor> target, int64_t k,
       else slots(std::integral_constant<int, 16>{});
       return;
     }
-    auto go = [&](auto nv) {
-      constexpr int NT = decltype(nv)::value, most = NT * kPer;
+    auto go = [&](auto nv, auto pv) {
+      constexpr int NT = decltype(nv)::value, PER = decltype(pv)::value;
+      constexpr int most = NT * PER;
       const int64_t splits = ceil_div(C, most);
       const int chunk = (int)ceil_div(ceil_div(C, splits), 16) * 16;
       TORCH_CHECK(rows * splits < INT32_MAX, "log_probs: too many rows");
@@ -727,7 +747,7 @@ log_probs_fwd(at::Tensor logits, c10::optional<at::Tensor> target, int64_t k,
       float* sp = splits > 1 ? sums.data_ptr<float>() : nullptr;
       uint64_t* kp =
           splits > 1 ? (uint64_t*)keys.data_ptr<int64_t>() : nullptr;
-      hipLaunchKernelGGL((log_probs_long_kernel<T, NT>), dim3(rows * splits),
+      hipLaunchKernelGGL((log_probs_long_kernel<T, NT, PER>), dim3(rows * splits),
                          dim3(NT), 0, stream, zp, zs, tp, ignore, (int)C,
                          (int)k, (int)splits, chunk, lpp,
                          ent.data_ptr<float>(), top_lp.data_ptr<float>(),
@@ -741,8 +761,9 @@ log_probs_fwd(at::Tensor logits, c10::optional<at::Tensor> target, int64_t k,
                            top_idx.data_ptr<int64_t>(),
                            stats.data_ptr<float>());
     };
-    if (C <= 256 * kPer) go(std::integral_constant<int, 256>{});
-    else go(std::integral_constant<int, 1024>{});
+    constexpr std::integral_constant<int, 16> per;
+    if (C <= 256 * 16) go(std::integral_constant<int, 256>{}, per);
+    else go(std::integral_constant<int, 1024>{}, per);
   });
   DOA_CHECK_HIP(hipGetLastError());
   return {lp, ent, top_lp, top_idx, stats};

@@ -679,7 +679,7 @@ log_probs_fwd(at::Tensor logits, c10::optional<at::Tensor> target, int64_t k,
   TORCH_CHECK(logits.is_cuda() && logits.dim() == 2,
               "log_probs: [rows, classes] GPU logits expected");
   const int64_t rows = logits.size(0), C = logits.size(1);
-  TORCH_CHECK(C >= 1 && C < INT32_MAX, "log_probs: 1 to 2^31 - 2 classes");
+  TORCH_CHECK(C >= 1 && C <= (1 << 30), "log_probs: 1 to 2^30 classes");
   TORCH_CHECK(k >= 0 && k <= kTopMost && k <= C, "log_probs: top_k is at most ",
               kTopMost, " and the number of classes, got ", k);
   if (target.has_value())

@@ -222,8 +222,8 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor> route_rows(at::Tensor ids,
   int bits = 0;
   while ((1 << bits) < G) ++bits;
   auto stream = stream_of_current();
-  // counters a block: 16384 ints (64 KiB of LDS), one set a wave
-  const int fit = std::max(1, kRouteMaxGroups / G);
+  // counters a block: 64 KiB of LDS with the scan's few, one set a wave
+  const int fit = std::max(1, (kRouteMaxGroups - 16) / G);
   auto go = [&](auto* idp) {
     using IdT = std::remove_const_t<std::remove_pointer_t<decltype(idp)>>;
     if (n <= 8192 && G <= 4096) {
@@ -269,6 +269,9 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor> route_rows(at::Tensor ids,
 // The row kernels: 2^sh lanes a row, 16 bytes a lane where rows allow it.
 // ---------------------------------------------------------------------------
 
+// a slot's row: not that of a dropped one, and never outside the sorted rows
+__device__ inline bool inside(int p, int64_t n) { return p >= 0 && p < n; }
+
 // rows behind the last group
 template <typename T, int V>
 __device__ inline void zero_tail(T* out, int64_t end, int64_t n, int D,
@@ -277,7 +280,8 @@ __device__ inline void zero_tail(T* out, int64_t end, int64_t n, int D,
   Vec<T, V> z;
 #pragma unroll
   for (int i = 0; i < V; ++i) z.v[i] = (T)0.f;
-  for (int64_t p = end + (((int64_t)blockIdx.x * blockDim.x + threadIdx.x) >> sh);
+  for (int64_t p = max((int64_t)0, end) +
+                   (((int64_t)blockIdx.x * blockDim.x + threadIdx.x) >> sh);
        p < n; p += ((int64_t)gridDim.x * blockDim.x) >> sh)
     for (int c = lane * V; c < D; c += V << sh)
       *reinterpret_cast<Vec<T, V>*>(out + p * D + c) = z;
@@ -297,7 +301,7 @@ __global__ __launch_bounds__(256) void dispatch_rows_kernel(
       const Vec<T, V> v = *reinterpret_cast<const Vec<T, V>*>(x + t * xs + c);
       for (int j = 0; j < k; ++j) {
         const int p = position[t * k + j];
-        if (p >= 0)
+        if (inside(p, rows * k))
           *reinterpret_cast<Vec<T, V>*>(out + (int64_t)p * D + c) = v;
       }
     }
@@ -320,7 +324,7 @@ __global__ __launch_bounds__(256) void combine_rows_kernel(
       for (int i = 0; i < V; ++i) acc[i] = 0.f;
       for (int j = 0; j < k; ++j) {
         const int p = position[t * k + j];
-        if (p < 0) continue;
+        if (!inside(p, rows * k)) continue;
         const float wj = w ? w[t * k + j] : 1.f;
         const Vec<T, V> v =
             *reinterpret_cast<const Vec<T, V>*>(y + (int64_t)p * ys + c);
@@ -351,7 +355,7 @@ __global__ __launch_bounds__(256) void combine_rows_bwd_kernel(
     for (int j = 0; j < k; ++j) {
       const int p = live ? position[t * k + j] : -1;
       float part = 0.f;
-      if (p >= 0) {
+      if (inside(p, rows * k)) {
         const float wj = w ? w[t * k + j] : 1.f;
         for (int c = lane * V; c < D; c += V << sh) {
           const Vec<T, V> gv =
@@ -404,6 +408,20 @@ static at::Tensor row_contiguous(const at::Tensor& t) {
              : t.contiguous();
 }
 
+static void check_plan(const at::Tensor& position, const char* what) {
+  TORCH_CHECK(position.dim() == 2 && position.scalar_type() == at::kInt &&
+                  position.is_contiguous(),
+              what, ": the plan's contiguous int32 positions expected");
+}
+static void check_plan(const at::Tensor& position, const at::Tensor& offsets,
+                       const char* what) {
+  check_plan(position, what);
+  TORCH_CHECK(offsets.dim() == 1 && offsets.scalar_type() == at::kLong &&
+                  offsets.numel() >= 1 && offsets.is_contiguous() &&
+                  offsets.device() == position.device(),
+              what, ": the plan's contiguous int64 offsets expected");
+}
+
 static void check_rows(const at::Tensor& t, const at::Tensor& position,
                        int64_t rows, const char* what) {
   TORCH_CHECK(t.is_cuda() && t.device() == position.device() && t.dim() == 2 &&
@@ -423,6 +441,7 @@ static const float* weights_ptr(const c10::optional<at::Tensor>& w,
 
 at::Tensor dispatch_rows(at::Tensor x, at::Tensor position,
                          at::Tensor offsets) {
+  check_plan(position, offsets, "dispatch_rows");
   const int64_t rows = position.size(0), k = position.size(1);
   check_rows(x, position, rows, "dispatch_rows");
   c10::DeviceGuard guard(x.device());
@@ -448,6 +467,7 @@ at::Tensor dispatch_rows(at::Tensor x, at::Tensor position,
 
 at::Tensor combine_rows(at::Tensor y, at::Tensor position,
                         c10::optional<at::Tensor> weights) {
+  check_plan(position, "combine_rows");
   const int64_t rows = position.size(0), k = position.size(1);
   check_rows(y, position, rows * k, "combine_rows");
   const float* wp = weights_ptr(weights, position, "combine_rows");
@@ -474,6 +494,7 @@ at::Tensor combine_rows(at::Tensor y, at::Tensor position,
 std::tuple<at::Tensor, at::Tensor> combine_rows_bwd(
     at::Tensor gout, c10::optional<at::Tensor> y, at::Tensor position,
     at::Tensor offsets, c10::optional<at::Tensor> weights, bool want_y) {
+  check_plan(position, offsets, "combine_rows");
   const int64_t rows = position.size(0), k = position.size(1);
   const bool want_w = y.has_value();
   check_rows(gout, position, rows, "combine_rows");

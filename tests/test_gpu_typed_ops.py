@@ -50,7 +50,7 @@ def strided(t, how):
 # ---------------------------------------------------------------------------
 @pytest.mark.parametrize("rows,k,groups", [
     (0, 2, 3), (1, 1, 1), (1, 2, 8), (63, 1, 5), (64, 3, 64), (1000, 2, 16),
-    (4096, 2, 4096), (8193, 1, 3), (20000, 2, 1345), (3000, 4, 16384),
+    (4096, 2, 4096), (4096, 2, 1024), (8193, 1, 3), (20000, 2, 1345), (3000, 4, 16384),
     (40000, 1, 5000),
 ])
 @pytest.mark.parametrize("dtype", [torch.int32, torch.int64])
@@ -89,6 +89,28 @@ def test_route_rows_refuses(dev):
         ops.dispatch_rows(route, torch.zeros(4, 2))
     with pytest.raises(AssertionError):
         ops.combine_rows(route, torch.zeros(4, 2, device=dev), torch.zeros(4))
+
+
+def test_plans_made_by_hand_stay_inside(dev):
+    """Positions that leave the sorted rows are dropped, never followed; other
+    layouts than the plan's own are refused."""
+    good = ops.route_rows(torch.tensor([[0, 1], [1, 0]], device=dev), 2)
+    x, y = torch.ones(2, 8, device=dev), torch.ones(4, 8, device=dev)
+    bad = good._replace(position=torch.tensor(
+        [[4, 2 ** 31 - 1], [-7, 0]], dtype=torch.int32, device=dev))
+    assert ops.dispatch_rows(bad, x).shape == (4, 8)
+    assert torch.equal(ops.combine_rows(bad, y)[:, 0].cpu(),
+                       torch.tensor([0.0, 1.0]))
+    yr, w = y.clone().requires_grad_(), torch.ones(2, 2, device=dev)
+    torch.autograd.grad(ops.combine_rows(bad, yr, w).sum(), yr)
+    torch.cuda.synchronize()
+    turned = good._replace(position=good.position.t())
+    for call in (lambda: ops.dispatch_rows(turned, x),
+                 lambda: ops.combine_rows(turned, y),
+                 lambda: ops.combine_rows(
+                     good._replace(position=good.position.long()), y)):
+        with pytest.raises(RuntimeError, match="the plan's contiguous"):
+            call()
 
 
 @pytest.mark.parametrize("rows,k,width", [

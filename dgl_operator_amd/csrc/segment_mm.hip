@@ -189,17 +189,13 @@ struct Tile {
 };
 
 template <typename T, typename Frag>
-__device__ inline f32x4 mma(Frag a, Frag b, f32x4 c) {
-  if constexpr (sizeof(T) == 4) {
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-      c = __builtin_amdgcn_mfma_f32_16x16x4f32(a[i], b[i], c, 0, 0, 0);
-    return c;
-  } else if constexpr (std::is_same_v<T, __bf16>) {
+__device__ inline f32x4 mma(Frag a, Frag b, f32x4 c, int q = 0) {
+  if constexpr (sizeof(T) == 4)
+    return __builtin_amdgcn_mfma_f32_16x16x4f32(a[q], b[q], c, 0, 0, 0);
+  else if constexpr (std::is_same_v<T, __bf16>)
     return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
-  } else {
+  else
     return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
-  }
 }
 
 // A wave's 16 FM x 16 FN results: strips of 16 rows go through `room` (ROOM
@@ -286,12 +282,15 @@ __device__ inline void tile_product(char* lds, const T* a, int64_t lda, int M,
       for (int i = 0; i < FM; ++i) fa[i] = read_a.get(la, i, kk);
 #pragma unroll
       for (int j = 0; j < FN; ++j) fb[j] = read_b.get(lb, j, kk);
+      // b first: a lane then holds 4 neighbouring columns of one row. fp32's
+      // four instructions a fragment go round the tiles, not on one of them
 #pragma unroll
-      for (int i = 0; i < FM; ++i)
+      for (int q = 0; q < (sizeof(T) == 4 ? 4 : 1); ++q)
 #pragma unroll
-        for (int j = 0; j < FN; ++j)
-          // b first: a lane then holds 4 neighbouring columns of one row
-          acc[i][j] = mma<T>(fb[j], fa[i], acc[i][j]);
+        for (int i = 0; i < FM; ++i)
+#pragma unroll
+          for (int j = 0; j < FN; ++j)
+            acc[i][j] = mma<T>(fb[j], fa[i], acc[i][j], q);
     }
   };
   int now = 0;
@@ -856,7 +855,8 @@ at::Tensor segment_mm(at::Tensor offsets, at::Tensor x, at::Tensor weight,
       if (R <= 48 * G)
         go(segment_mm_kernel<T, WC, W, 32, 64, 1, 4, 128, 2>, 32, 64, 256);
       else if constexpr (sizeof(T) == 4)
-        go(segment_mm_kernel<T, WC, W, 64, 64, 2, 2, 128, 2>, 64, 64, 256);
+        go(segment_mm_kernel<T, WC, W, 64, 64, 2, 2, W ? 64 : 128, W ? 6 : 2>,
+           64, 64, 256);
       else if (R <= 96 * G)
         go(segment_mm_kernel<T, WC, W, 64, 128, 2, 2, 128, 2>, 64, 128, 256);
       else if constexpr (W)

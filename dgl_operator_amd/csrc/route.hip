@@ -8,6 +8,11 @@
 // is a sum of integers or of floats in a fixed order, so a run repeats bit
 // for bit. No host synchronisation: the number of kept slots stays on the
 // device.
+//
+// Measured on one MI355X, where a large copy moves 4.8 TB/s: the plan of 53504
+// slots in 16 groups 12 us in three launches, of 16 slots 3 us in one, of 65536
+// slots in 1345 groups 32 us (there each wave's own start of every group is
+// what counts).
 
 #include "vec.h"
 
@@ -267,6 +272,10 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor> route_rows(at::Tensor ids,
 
 // ---------------------------------------------------------------------------
 // The row kernels: 2^sh lanes a row, 16 bytes a lane where rows allow it.
+// Bound by memory. They go over the rows before sorting, so that each of those
+// is read (or written) once whatever k, and the sorted rows once each. 262144
+// rows of 512 in bf16 with k = 2: copy out 132 us (6.1 TB/s), weighted sum 157 us
+// (5.1 TB/s), its gradient 257 us (5.2 TB/s).
 // ---------------------------------------------------------------------------
 
 // a slot's row: not that of a dropped one, and never outside the sorted rows

@@ -125,26 +125,41 @@ struct Tile {
       }
     }
   }
-  // the same through registers, element by element where a chunk is cut
+  // The same through registers, from any element's address: a chunk that the
+  // operand's edge cuts is read whole and masked, unless that would leave its
+  // memory, which ends at `end`.
   static __device__ void fetch(const T* p, int64_t ld, int side, int64_t depth,
-                               Chunk* to) {
+                               const T* end, Chunk* to) {
     const int O = COL ? (int)min((int64_t)BK, depth) : side;
     const int I = COL ? side : (int)min((int64_t)BK, depth);
+    using Bits = std::conditional_t<sizeof(T) == 2, uint16_t, uint32_t>;
+    constexpr int W = 4 / sizeof(T);  // elements a word
 #pragma unroll
     for (int i = 0; i < PER; ++i) {
       const int id = i * THREADS + threadIdx.x, o = id / CHUNKS;
       const int c = swizzle<T, COL, CHUNKS>(id % CHUNKS, o) * E;
+      const int there = o < O ? I - c : 0;  // elements of the chunk there are
       const T* src = p + o * ld + c;
-      union { Chunk q; T v[E]; } u;
-      u.q = Chunk{0, 0, 0, 0};
-      if (o < O && c + E <= I) {
-        u.q = *reinterpret_cast<const LooseChunk*>(src);
-      } else if (o < O) {
+      Chunk q = {0, 0, 0, 0};
+      if (there > 0) {
+        if (src + E <= end) {
+          q = *reinterpret_cast<const LooseChunk*>(src);
+        } else {
 #pragma unroll
-        for (int e = 0; e < E; ++e)
-          if (c + e < I) u.v[e] = src[e];
+          for (int e = 0; e < E; ++e)
+            if (e < there)
+              q[e / W] |= (uint32_t)reinterpret_cast<const Bits*>(src)[e]
+                          << (e % W * 16);
+        }
+        if (there < E) {
+#pragma unroll
+          for (int w = 0; w < 4; ++w) {
+            const int in = there - w * W;  // of this word
+            q[w] &= in >= W ? ~0u : in == 1 && W == 2 ? 0xffffu : 0u;
+          }
+        }
       }
-      to[i] = u.q;
+      to[i] = q;
     }
   }
   static __device__ void put(const Chunk* from, char* lds) {
@@ -269,8 +284,9 @@ constexpr int lds_bytes(int BM, int BN, int STEP) { return 2 * (BM + BN) * STEP;
 template <typename T, typename O, bool AC, bool BC, bool WHOLE, int BM, int BN,
           int WM, int WN, int STEP>
 __device__ inline void tile_product(char* lds, const T* a, int64_t lda, int M,
-                                    const T* b, int64_t ldb, int N, int64_t K,
-                                    O* c, int64_t ldc) {
+                                    const T* end_a, const T* b, int64_t ldb,
+                                    int N, const T* end_b, int64_t K, O* c,
+                                    int64_t ldc) {
   constexpr int THREADS = 64 * WM * WN;
   using TA = Tile<T, AC, BM, THREADS, STEP>;
   using TB = Tile<T, BC, BN, THREADS, STEP>;
@@ -330,8 +346,8 @@ __device__ inline void tile_product(char* lds, const T* a, int64_t lda, int M,
   } else {
     Chunk ra[TA::PER], rb[TB::PER];
     if (K > 0) {
-      TA::fetch(a, lda, M, K, ra);
-      TB::fetch(b, ldb, N, K, rb);
+      TA::fetch(a, lda, M, K, end_a, ra);
+      TB::fetch(b, ldb, N, K, end_b, rb);
       TA::put(ra, lds);
       TB::put(rb, lds + TA::BYTES);
     }
@@ -340,8 +356,8 @@ __device__ inline void tile_product(char* lds, const T* a, int64_t lda, int M,
       if (left > BK) {
         a += step_a;
         b += step_b;
-        TA::fetch(a, lda, M, left - BK, ra);
-        TB::fetch(b, ldb, N, left - BK, rb);
+        TA::fetch(a, lda, M, left - BK, end_a, ra);
+        TB::fetch(b, ldb, N, left - BK, end_b, rb);
       }
       multiply(lds + now * STAGE, lds + now * STAGE + TA::BYTES, left);
       if (left > BK) {
@@ -413,8 +429,10 @@ __global__ __launch_bounds__(64 * WM * WN, WAVES) void segment_mm_kernel(
   if (s.many == 0) return;
   const int n0 = work % tiles_n * BN;
   tile_product<T, T, false, WC, WHOLE, BM, BN, WM, WN, STEP>(
-      lds, x + s.r0 * xs, xs, s.many, w + s.g * wg + n0 * (WC ? 1 : wl), wl,
-      min(BN, N - n0), K, y + (int64_t)s.r0 * N + n0, N);
+      lds, x + s.r0 * xs, xs, s.many, x + (rows - 1) * xs + K,
+      w + s.g * wg + n0 * (WC ? 1 : wl), wl, min(BN, N - n0),
+      w + (G - 1) * wg + ((WC ? K : N) - 1) * wl + (WC ? N : K), K,
+      y + (int64_t)s.r0 * N + n0, N);
 }
 
 // ---------------------------------------------------------------------------
@@ -725,8 +743,9 @@ __global__ __launch_bounds__(64 * WM * WN, WAVES) void segment_wgrad_kernel(
   const int64_t begin = offset_at(offsets, e, rows);
   const int64_t len = offset_at(offsets, e + 1, rows) - begin;
   tile_product<T, T, true, true, WHOLE, BM, BN, WM, WN, STEP>(
-      lds, x + begin * xs + k0, xs, min(BM, K - k0), g + begin * gs + n0, gs,
-      min(BN, N - n0), len, dw + ((int64_t)e * K + k0) * N + n0, N);
+      lds, x + begin * xs + k0, xs, min(BM, K - k0), x + (rows - 1) * xs + K,
+      g + begin * gs + n0, gs, min(BN, N - n0), g + (rows - 1) * gs + N, len,
+      dw + ((int64_t)e * K + k0) * N + n0, N);
 }
 
 // dW by teams, as segment_wgrad_wide_kernel: few groups with many rows
@@ -757,11 +776,11 @@ __global__ __launch_bounds__(64 * WM * WN, WAVES) void segment_wgrad_teams_kerne
     __syncthreads();  // the last product's LDS is free
     if (r == g_start && stop == g_stop)
       tile_product<T, T, true, true, WHOLE, BM, BN, WM, WN, STEP>(
-          lds, a, xs, min(BM, K - k0), b, gs, min(BN, N - n0), stop - r,
+          lds, a, xs, min(BM, K - k0), x + (rows - 1) * xs + K, b, gs, min(BN, N - n0), g + (rows - 1) * gs + N, stop - r,
           dw + (int64_t)e * K * N + corner, N);
     else
       tile_product<T, float, true, true, WHOLE, BM, BN, WM, WN, STEP>(
-          lds, a, xs, min(BM, K - k0), b, gs, min(BN, N - n0), stop - r,
+          lds, a, xs, min(BM, K - k0), x + (rows - 1) * xs + K, b, gs, min(BN, N - n0), g + (rows - 1) * gs + N, stop - r,
           planes + (2 * (int64_t)team + (r == g_start)) * K * N + corner, N);
     r = stop;
   }
@@ -874,10 +893,9 @@ at::Tensor segment_mm(at::Tensor offsets, at::Tensor x, at::Tensor weight,
            64, 64, 256);
       else if (R <= 96 * G)
         go(segment_mm_kernel<T, WC, W, 64, 128, 2, 2, 128, 2>, 64, 128, 256);
-      else if constexpr (W)
-        go(segment_mm_kernel<T, WC, W, 128, 128, 2, 2, 64, 4>, 128, 128, 256);
       else
-        go(segment_mm_kernel<T, WC, W, 128, 128, 2, 2, 128, 2>, 128, 128, 256);
+        go(segment_mm_kernel<T, WC, W, 128, 128, 2, 2, 64, W ? 4 : 2>, 128, 128,
+           256);
     };
     if (wc)
       whole ? pick(std::true_type{}, std::true_type{})
@@ -938,15 +956,18 @@ at::Tensor segment_mm_wgrad(at::Tensor offsets, at::Tensor x, at::Tensor grad) {
     }
     auto pick = [&](auto wv) {
       constexpr bool W = decltype(wv)::value;
-      constexpr int B = sizeof(T) == 4 ? 64 : 128;
+      constexpr int B = W && sizeof(T) == 2 ? 128 : 64;
       const int64_t tk = ceil_div(K, B), tn = ceil_div(N, B), tiles = tk * tn;
-      // Where groups and tiles alone are fewer than two blocks a CU: teams, of
-      // rows enough that a team reads as much as its plane costs (8 bytes an
-      // element, written and read).
-      const int64_t each = std::max<int64_t>(256, 2 * K * N / (K + N));
+      // Teams where groups are long and, with their tiles, few: their lengths
+      // differ, and the longest would be waited for. A team has rows enough to
+      // read as much as its plane costs (8 bytes an element, written and read);
+      // as many blocks as the chip holds, two a CU or four of the small tiles.
+      const int64_t blocks = (B == 64 ? 4 : 2) * cus;
+      const int64_t each =
+          std::max<int64_t>(B == 64 ? 512 : 256, 2 * K * N / (K + N));
       const int64_t teams =
-          std::min(ceil_div(2 * cus, tiles), ceil_div(R, each));
-      if (tiles * G < 2 * cus && teams > G) {
+          std::min(ceil_div(blocks, tiles), ceil_div(R, each));
+      if (teams > 1 && R >= 256 * G && tiles * G < 8 * blocks) {
         by_teams(segment_wgrad_teams_kernel<T, W, B, B, 2, 2, 128, 2>,
                  (int)(teams * tiles), 256, B, tiles, (int)teams);
         return;

@@ -732,6 +732,7 @@ log_probs_fwd(at::Tensor logits, c10::optional<at::Tensor> target, int64_t k,
         else if (k == 1) go(lv, std::integral_constant<int, 1>{});
         else if (k <= 5) go(lv, std::integral_constant<int, 5>{});
         else if (k <= 10) go(lv, std::integral_constant<int, 10>{});
+        else if (k <= 16) go(lv, std::integral_constant<int, 16>{});
         else go(lv, std::integral_constant<int, kTopMost>{});
       };
       if (L == 1) slots(std::integral_constant<int, 1>{});

@@ -318,7 +318,7 @@ def test_log_probs_sizes(dev, rows, C, dtype):
         z.masked_fill_(hide, -math.inf)
     z = z.to(dtype)
     t = torch.randint(0, C, (rows,))
-    for k in {0, 1, min(C, 5), min(C, 10), min(C, 32)}:
+    for k in {0, 1, min(C, 5), min(C, 10), min(C, 15), min(C, 20), min(C, 32)}:
         check_log_probs(dev, z, t, k)
     check_log_probs(dev, z, None, min(C, 3))
 
@@ -521,6 +521,48 @@ def test_mixture_on_another_stream(dev):
     s.synchronize()
     for g in got:
         assert torch.equal(g, want)
+
+
+def test_mixture_on_two_streams_at_once(dev):
+    """Two programs side by side share nothing."""
+    ins = [[t.to(dev) for t in mixture_inputs(n)] for n in (400, 900)]
+    want = [mixture(None, *i, 6, 2)[0] for i in ins]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in ins]
+    got = [[], []]
+    for _ in range(5):
+        for n, s in enumerate(streams):
+            with torch.cuda.stream(s):
+                got[n].append(mixture(None, *ins[n], 6, 2)[0])
+    torch.cuda.synchronize()
+    for g, w in zip(got, want):
+        for t in g:
+            assert torch.equal(t, w)
+
+
+def test_gradients_of_one_side_and_shared_weights(dev):
+    """Each input's gradient alone; one weight expanded over all groups, whose
+    gradient is the sum over them; an output's gradient that is a broadcast."""
+    offsets = offsets_of([700, 1, 0, 340]).to(dev)
+    x = torch.randn(1041, 136, device=dev).bfloat16()
+    w = (torch.randn(136, 264, device=dev) / 12).bfloat16()
+    for need_x, need_w in ((True, False), (False, True)):
+        xd = x.clone().requires_grad_(need_x)
+        wd = w.clone().requires_grad_(need_w)
+        y = ops.segment_mm(offsets, xd, wd.expand(4, 136, 264))
+        within(y, oracle.matmul(x.cpu(), w.cpu(), x.dtype))
+        g, = torch.autograd.grad(y, xd if need_x else wd,
+                                 torch.ones(1, 1, device=dev).bfloat16()
+                                 .expand(1041, 264))
+        ones = torch.ones(1041, 264).bfloat16()
+        if need_x:
+            within(g, oracle.matmul(ones, w.cpu().t(), x.dtype))
+        else:
+            ref, tol = oracle.matmul(x.cpu().t(), ones, x.dtype)
+            # four groups' gradients, each rounded, and their sum rounded
+            # thrice: at most 4 + 3 halves of a step of sums of |x|
+            size = x.cpu().double().abs().sum(0)[:, None]
+            within(g, (ref, tol + 7 * oracle.half(x.dtype) * size))
 
 
 def test_mixture_captured(dev):

@@ -495,10 +495,12 @@ __global__ __launch_bounds__(256) void log_probs_join_kernel(
   for (int p = threadIdx.x; p < splits; p += 256) {
     // sums over a base of their own: e^(z - m_p) -> e^(z - m)
     const float mp = ps[3 * p];
+    // (a part that lies far below has e = 0; its d times its sum, a part's length
+    // at most, must not pass the largest float there)
     const float d = (mp == -INFINITY ? 0.f : mp) - base;
     const float e = ps[3 * p + 1] == 0.f ? 0.f : __expf(d);
     s += ps[3 * p + 1] * e;
-    a += (ps[3 * p + 2] + d * ps[3 * p + 1]) * e;
+    a += (ps[3 * p + 2] + fmaxf(d, -1e30f) * ps[3 * p + 1]) * e;
   }
   s = over_block(s, [](float x, float y) { return x + y; });
   a = over_block(a, [](float x, float y) { return x + y; });

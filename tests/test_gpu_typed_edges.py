@@ -1,0 +1,46 @@
+"""Calls at the edges of the typed-row operators and of log_probs on the GPU:
+finite masks that fill a part of a long row, large gradients, empty batches,
+launches of more threads than one grid holds, gradients that nobody asked for."""
+import math
+
+import pytest
+import torch
+
+import typed_oracle as oracle
+from test_typed_ops import check_log_probs
+
+from dgl_operator_amd import ops
+from dgl_operator_amd.ops import backend
+
+pytestmark = pytest.mark.gpu
+
+TYPES = [torch.float32, torch.bfloat16, torch.float16]
+
+
+@pytest.fixture(scope="module")
+def dev():
+    assert torch.cuda.is_available()
+    assert backend.has_extension(), "HIP extension must be built on GPU boxes"
+    return torch.device("cuda:0")
+
+
+@pytest.mark.parametrize("C", [16400, 20000, 40001])
+@pytest.mark.parametrize("dtype", TYPES)
+def test_parts_of_a_long_row_far_apart(dev, C, dtype):
+    """Parts of a split row whose values lie as far apart as the type lets them:
+    a range of classes masked by the lowest value, at either end or in the
+    middle, a row that is lowest but for one, one that is highest but for one."""
+    low, high = torch.finfo(dtype).min, torch.finfo(dtype).max
+    z = torch.randn(6, C)
+    z[0, C // 2 - 16:] = low
+    z[1, :C // 2 + 16] = low
+    z[2, C // 3:C - C // 3] = low
+    z[3] = low
+    z[3, C - 1] = 1.0
+    z[4] = high
+    z[4, 0] = low
+    z[5, :C - 8] = -math.inf
+    z = z.to(dtype)
+    t = torch.tensor([3, C - 2, 1, C - 1, 7, C - 3])
+    for k in (0, 5):
+        check_log_probs(dev, z, t, k)

@@ -632,7 +632,9 @@ __global__ __launch_bounds__(256) void log_probs_bwd_kernel(
     for (int e = 0; e < E; ++e) {
       const RowPull& u = info[r];
       const float l = ((float)part[q].e[e] - u.base) - u.logs;
-      const float v = -__expf(l) * (u.pull + u.gh * (fmaxf(l, -1e30f) + u.ent));
+      // (e^-128 is 0 in fp32: from there on l must not spoil the product, however
+      // large gh is)
+      const float v = -__expf(l) * (u.pull + u.gh * (fmaxf(l, -128.f) + u.ent));
       g.e[e] = u.logs == INFINITY ? 0.f : v;
       // (behind the last row: any row there is)
       if (++c == W) c = 0, r = min(r + 1, many - 1);

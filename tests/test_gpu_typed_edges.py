@@ -44,3 +44,22 @@ def test_parts_of_a_long_row_far_apart(dev, C, dtype):
     t = torch.tensor([3, C - 2, 1, C - 1, 7, C - 3])
     for k in (0, 5):
         check_log_probs(dev, z, t, k)
+
+
+@pytest.mark.parametrize("C", [20, 300, 5000, 20000])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_large_entropy_gradients(dev, C, dtype):
+    """A scaled loss: the gradient is linear in the entropy's, so that a power
+    of two goes through it exactly, also where a class was taken away."""
+    z = torch.randn(5, C)
+    z[:, ::3] = -math.inf
+    z[1] = torch.finfo(dtype).min
+    z[1, 4] = 0.0
+    z[2] = -math.inf
+    zd = z.to(dtype).to(dev).requires_grad_()
+    ent = ops.log_probs(zd).entropy
+    small, = torch.autograd.grad(ent, zd, torch.ones_like(ent),
+                                 retain_graph=True)
+    large, = torch.autograd.grad(ent, zd, torch.full_like(ent, 2.0 ** 33))
+    assert torch.isfinite(large).all()
+    assert torch.equal(large, small * 2.0 ** 33)

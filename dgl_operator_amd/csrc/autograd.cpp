@@ -82,7 +82,6 @@ struct CombineRows : Function<CombineRows> {
     at::Tensor w;
     if (weights.has_value()) w = weights->to(at::kFloat).contiguous();
     const bool want_w = weights.has_value() && weights->requires_grad();
-    ctx->saved_data["want_y"] = y.requires_grad();
     if (weights.has_value())
       ctx->saved_data["type"] = (int64_t)weights->scalar_type();
     ctx->save_for_backward({want_w ? y : Variable(), w, position, offsets});
@@ -95,9 +94,11 @@ struct CombineRows : Function<CombineRows> {
     {
       at::AutoGradMode off(false);
       const auto s = ctx->get_saved_variables();
-      auto [dy, dw] = combine_rows_bwd(g[0], maybe(s[0]), s[2], s[3],
-                                       maybe(s[1]),
-                                       ctx->saved_data["want_y"].toBool());
+      // y has the graph's first edge, the weights, if there are any, its second
+      const bool want_y = ctx->needs_input_grad(0);
+      const bool want_w = s[0].defined() && ctx->needs_input_grad(1);
+      auto [dy, dw] = combine_rows_bwd(g[0], want_w ? Maybe(s[0]) : Maybe(),
+                                       s[2], s[3], maybe(s[1]), want_y);
       out[0] = dy;
       if (dw.defined())
         out[1] = dw.to((at::ScalarType)ctx->saved_data["type"].toInt());
@@ -120,8 +121,11 @@ struct SegmentMM : Function<SegmentMM> {
     {
       at::AutoGradMode off(false);
       const auto s = ctx->get_saved_variables();
-      if (s[2].defined()) out[1] = segment_mm(s[0], g[0], s[2], true);
-      if (s[1].defined()) out[2] = segment_mm_wgrad(s[0], s[1], g[0]);
+      // (the graph's edges: offsets, x, weight)
+      if (s[2].defined() && ctx->needs_input_grad(1))
+        out[1] = segment_mm(s[0], g[0], s[2], true);
+      if (s[1].defined() && ctx->needs_input_grad(2))
+        out[2] = segment_mm_wgrad(s[0], s[1], g[0]);
     }
     return once(std::move(out));
   }

@@ -63,3 +63,43 @@ def test_large_entropy_gradients(dev, C, dtype):
     large, = torch.autograd.grad(ent, zd, torch.full_like(ent, 2.0 ** 33))
     assert torch.isfinite(large).all()
     assert torch.equal(large, small * 2.0 ** 33)
+
+
+def peak_of(call):
+    """Bytes that a call holds at most beyond what was there."""
+    torch.cuda.synchronize()
+    before = torch.cuda.memory_allocated()
+    torch.cuda.reset_peak_memory_stats()
+    out = call()
+    torch.cuda.synchronize()
+    return out, torch.cuda.max_memory_allocated() - before
+
+
+def test_gradients_that_nobody_asks_for(dev):
+    """Both inputs may learn; a backward pass makes the gradients asked for and
+    does not hold the others'."""
+    offsets = torch.tensor([0, 100, 400], device=dev)
+    x = torch.randn(400, 512, device=dev, requires_grad=True)
+    w = torch.randn(2, 512, 4096, device=dev, requires_grad=True)
+    y = ops.segment_mm(offsets, x, w)
+    g = torch.ones_like(y)
+    (dx,), held = peak_of(lambda: torch.autograd.grad(y, x, g, retain_graph=True))
+    assert held < 2 * x.numel() * 4, "dw is 16 times dx"
+    both = torch.autograd.grad(y, (x, w), g, retain_graph=True)
+    assert torch.equal(dx, both[0])
+    (dw,), _ = peak_of(lambda: torch.autograd.grad(y, w, g))
+    assert torch.equal(dw, both[1])
+
+    ids = torch.randint(0, 4, (3000, 2), device=dev)
+    route = ops.route_rows(ids, 4)
+    rows = torch.randn(6000, 256, device=dev, requires_grad=True)
+    weights = torch.rand(3000, 2, device=dev, requires_grad=True)
+    out = ops.combine_rows(route, rows, weights)
+    g = torch.randn_like(out)
+    (dweights,), held = peak_of(
+        lambda: torch.autograd.grad(out, weights, g, retain_graph=True))
+    assert held < rows.numel() * 4 // 2
+    (drows,), _ = peak_of(
+        lambda: torch.autograd.grad(out, rows, g, retain_graph=True))
+    both = torch.autograd.grad(out, (rows, weights), g)
+    assert torch.equal(drows, both[0]) and torch.equal(dweights, both[1])

@@ -186,14 +186,15 @@ class Manager:
 
                 print(f"[manager] reconcile error for {key}: {e}")
                 traceback.print_exc()
-                continue
-            if job.deletion_timestamp is not None:
-                del self.jobs[key]
-                self._written_statuses.pop(key, None)
-            elif self.watch_crs:
-                self._write_status(job)
+            else:
+                if job.deletion_timestamp is not None:
+                    del self.jobs[key]
+                    self._written_statuses.pop(key, None)
+                elif self.watch_crs:
+                    self._write_status(job)
             # the lease is good for a ttl from its renewal: a pass that takes
-            # longer (many kubectl calls a job) must not let a standby in
+            # longer (many kubectl calls a job, a job that runs into their
+            # time limits) must not let a standby in, nor go on beside one
             if not self._ensure_leadership():
                 return
 

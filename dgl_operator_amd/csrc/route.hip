@@ -247,7 +247,8 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor> route_rows(at::Tensor ids,
     const int64_t want =
         std::max<int64_t>({256, G / 4, ceil_div(n, 8192)});
     const int tile = (int)ceil_div(want, 64) * 64;
-    const int tiles = (int)ceil_div(n, tile);
+    // (one tile where there is no slot: it writes the offsets)
+    const int tiles = (int)std::max<int64_t>(1, ceil_div(n, tile));
     auto counts = at::empty({(int64_t)G * tiles + G}, i32);
     int* cp = counts.data_ptr<int>();
     int* totals = cp + (int64_t)G * tiles;

@@ -103,3 +103,24 @@ def test_gradients_that_nobody_asks_for(dev):
         lambda: torch.autograd.grad(out, rows, g, retain_graph=True))
     both = torch.autograd.grad(out, (rows, weights), g)
     assert torch.equal(drows, both[0]) and torch.equal(dweights, both[1])
+
+
+@pytest.mark.parametrize("groups", [1, 3, 4096, 4097, 5000, 16384])
+@pytest.mark.parametrize("dtype", [torch.int32, torch.int64])
+def test_no_slots(dev, groups, dtype):
+    """An empty batch, however many groups there are, and the operators on it."""
+    for k in (1, 2):
+        ids = torch.empty(0, k, dtype=dtype, device=dev)
+        # the block that the offsets take next is not zero by chance
+        del_me = torch.full((groups + 1,), 7, device=dev)
+        del del_me
+        route = ops.route_rows(ids, groups)
+        assert route.offsets.shape == (groups + 1,) and not route.offsets.any()
+        assert route.position.shape == (0, k) and route.source.shape == (0,)
+        x = torch.zeros(0, 8, device=dev, requires_grad=True)
+        w = torch.ones(groups, 8, 4, device=dev, requires_grad=True)
+        y = ops.segment_mm(route.offsets, ops.dispatch_rows(route, x), w)
+        out = ops.combine_rows(route, y)
+        assert out.shape == (0, 4)
+        dx, dw = torch.autograd.grad(out.sum(), (x, w))
+        assert dx.shape == (0, 8) and not dw.any()

@@ -241,3 +241,12 @@ def test_log_probs_refusals():
     for k in (-1, 5):
         with pytest.raises(AssertionError):
             ops.log_probs(z, None, top_k=k)
+
+
+@pytest.mark.parametrize("groups", [1, 5000, 16384])
+def test_no_slots(groups):
+    route = ops.route_rows(torch.empty(0, 2, dtype=torch.int64), groups)
+    assert route.offsets.shape == (groups + 1,) and not route.offsets.any()
+    assert route.position.shape == (0, 2) and route.source.shape == (0,)
+    out = ops.combine_rows(route, ops.dispatch_rows(route, torch.zeros(0, 8)))
+    assert out.shape == (0, 8)

@@ -677,6 +677,14 @@ __global__ __launch_bounds__(256) void log_probs_bwd_kernel(
   }
 }
 
+// more rows than one grid has threads for go out in launches of `most` rows, one
+// behind the other on the stream
+template <typename Launch>
+static void by_grids(int64_t rows, int64_t most, Launch launch) {
+  for (int64_t r0 = 0; r0 < rows; r0 += most)
+    launch(r0, std::min(most, rows - r0));
+}
+
 static at::Tensor logits_rows(const at::Tensor& z) {
   return (z.size(1) <= 1 || z.stride(1) == 1) && z.stride(0) >= 0
              ? z
@@ -707,12 +715,25 @@ log_probs_fwd(at::Tensor logits, c10::optional<at::Tensor> target, int64_t k,
   auto top_idx = at::empty({rows, k}, logits.options().dtype(at::kLong));
   auto stats = at::empty({rows, 2}, f32);
   if (rows == 0) return {lp, ent, top_lp, top_idx, stats};
-  const int64_t* tp = target.has_value() ? target->data_ptr<int64_t>() : nullptr;
-  float* lpp = lp.defined() ? lp.data_ptr<float>() : nullptr;
   auto stream = stream_of_current();
   DOA_FLOAT_TYPES(logits.scalar_type(), "log_probs", [&] {
-    const T* zp = (const T*)zc.data_ptr();
     const int64_t zs = zc.stride(0);
+    // rows r0 .. r0 + n of everything there is a row of
+    struct Rows {
+      const T* z;
+      const int64_t* target;
+      float *lp, *ent, *top_lp;
+      int64_t* top_idx;
+      float* stats;
+    };
+    auto rows_from = [&](int64_t r0) {
+      return Rows{(const T*)zc.data_ptr() + r0 * zs,
+                  target.has_value() ? target->data_ptr<int64_t>() + r0 : nullptr,
+                  lp.defined() ? lp.data_ptr<float>() + r0 : nullptr,
+                  ent.data_ptr<float>() + r0, top_lp.data_ptr<float>() + r0 * k,
+                  top_idx.data_ptr<int64_t>() + r0 * k,
+                  stats.data_ptr<float>() + r0 * 2};
+    };
     const int64_t row_bytes = C * sizeof(T);
     if (row_bytes <= 2048) {
       // lanes a row: as many as keep a wave's rows at 8 KiB of LDS, more where
@@ -720,16 +741,17 @@ log_probs_fwd(at::Tensor logits, c10::optional<at::Tensor> target, int64_t k,
       int L = row_bytes <= 128 ? 1 : row_bytes <= 512 ? 4 : 16;
       while (L < 16 && rows * L < 64 * 1024) L *= 4;
       const int wave_bytes = (int)ceil_div(64 / L * row_bytes, 16) * 16;
-      const int64_t blocks = ceil_div(rows, 4 * (64 / L));
-      TORCH_CHECK(blocks < INT32_MAX, "log_probs: too many rows");
+      const int64_t per_block = 4 * (64 / L);
       auto go = [&](auto lv, auto kv) {
-        hipLaunchKernelGGL(
-            (log_probs_short_kernel<T, decltype(lv)::value,
-                                    decltype(kv)::value>),
-            dim3(blocks), dim3(256), 4 * wave_bytes, stream, zp, zs, tp, ignore,
-            rows, (int)C, (int)k, lpp, ent.data_ptr<float>(),
-            top_lp.data_ptr<float>(), top_idx.data_ptr<int64_t>(),
-            stats.data_ptr<float>(), wave_bytes);
+        by_grids(rows, kMostThreads / 256 * per_block, [&](int64_t r0, int64_t n) {
+          const Rows r = rows_from(r0);
+          hipLaunchKernelGGL(
+              (log_probs_short_kernel<T, decltype(lv)::value,
+                                      decltype(kv)::value>),
+              dim3(ceil_div(n, per_block)), dim3(256), 4 * wave_bytes, stream,
+              r.z, zs, r.target, ignore, n, (int)C, (int)k, r.lp, r.ent,
+              r.top_lp, r.top_idx, r.stats, wave_bytes);
+        });
       };
       auto slots = [&](auto lv) {  // registers for the next such number of keys
         if (k == 0) go(lv, std::integral_constant<int, 0>{});
@@ -749,28 +771,28 @@ log_probs_fwd(at::Tensor logits, c10::optional<at::Tensor> target, int64_t k,
       constexpr int most = NT * PER;
       const int64_t splits = ceil_div(C, most);
       const int chunk = (int)ceil_div(ceil_div(C, splits), 16) * 16;
-      TORCH_CHECK(rows * splits < INT32_MAX, "log_probs: too many rows");
+      const int64_t grid = kMostThreads / (NT * splits);
       at::Tensor sums, keys;
       if (splits > 1) {
-        sums = at::empty({rows * splits * 3}, f32);
-        keys = at::empty({rows * splits * k}, top_idx.options());
+        const int64_t parts = std::min(rows, grid) * splits;
+        sums = at::empty({parts * 3}, f32);
+        keys = at::empty({parts * k}, top_idx.options());
       }
       float* sp = splits > 1 ? sums.data_ptr<float>() : nullptr;
       uint64_t* kp =
           splits > 1 ? (uint64_t*)keys.data_ptr<int64_t>() : nullptr;
-      hipLaunchKernelGGL((log_probs_long_kernel<T, NT, PER>), dim3(rows * splits),
-                         dim3(NT), 0, stream, zp, zs, tp, ignore, (int)C,
-                         (int)k, (int)splits, chunk, lpp,
-                         ent.data_ptr<float>(), top_lp.data_ptr<float>(),
-                         top_idx.data_ptr<int64_t>(), stats.data_ptr<float>(),
-                         sp, kp);
-      if (splits > 1)
-        hipLaunchKernelGGL((log_probs_join_kernel<T>), dim3(rows), dim3(256), 0,
-                           stream, zp, zs, tp, ignore, (int)C, (int)k,
-                           (int)splits, sp, kp, lpp, ent.data_ptr<float>(),
-                           top_lp.data_ptr<float>(),
-                           top_idx.data_ptr<int64_t>(),
-                           stats.data_ptr<float>());
+      by_grids(rows, grid, [&](int64_t r0, int64_t n) {
+        const Rows r = rows_from(r0);
+        hipLaunchKernelGGL((log_probs_long_kernel<T, NT, PER>), dim3(n * splits),
+                           dim3(NT), 0, stream, r.z, zs, r.target, ignore, (int)C,
+                           (int)k, (int)splits, chunk, r.lp, r.ent, r.top_lp,
+                           r.top_idx, r.stats, sp, kp);
+        if (splits > 1)
+          hipLaunchKernelGGL((log_probs_join_kernel<T>), dim3(n), dim3(256), 0,
+                             stream, r.z, zs, r.target, ignore, (int)C, (int)k,
+                             (int)splits, sp, kp, r.lp, r.ent, r.top_lp,
+                             r.top_idx, r.stats);
+      });
     };
     constexpr std::integral_constant<int, 16> per;
     if (C <= 256 * 16) go(std::integral_constant<int, 256>{}, per);
@@ -806,17 +828,21 @@ at::Tensor log_probs_bwd(at::Tensor logits, c10::optional<at::Tensor> target,
   // rows a tile: what fits, but at least 1024 tiles where there are the rows
   const int64_t tile_rows = std::max<int64_t>(
       1, std::min<int64_t>({kTileRows, kTileElems / W, ceil_div(rows, 1024)}));
-  const int64_t blocks = ceil_div(rows, tile_rows) * col_tiles;
-  TORCH_CHECK(blocks < INT32_MAX, "log_probs: too many rows");
   const uint64_t magic = ((uint64_t)1 << 32) / W + 1;
   DOA_FLOAT_TYPES(logits.scalar_type(), "log_probs", [&] {
-    hipLaunchKernelGGL(
-        (log_probs_bwd_kernel<T>), dim3(blocks), dim3(256), 0,
-        stream_of_current(), (const T*)zc.data_ptr(), zc.stride(0),
-        target.has_value() ? target->data_ptr<int64_t>() : nullptr, ignore,
-        top_idx.data_ptr<int64_t>(), stats.data_ptr<float>(),
-        ent.data_ptr<float>(), gp[0], gp[1], gp[2], rows, (int)C, (int)k,
-        (int)tile_rows, (int)col_tiles, magic, (T*)dz.data_ptr());
+    by_grids(rows, kMostThreads / 256 / col_tiles * tile_rows,
+             [&](int64_t r0, int64_t n) {
+      hipLaunchKernelGGL(
+          (log_probs_bwd_kernel<T>), dim3(ceil_div(n, tile_rows) * col_tiles),
+          dim3(256), 0, stream_of_current(),
+          (const T*)zc.data_ptr() + r0 * zc.stride(0), zc.stride(0),
+          target.has_value() ? target->data_ptr<int64_t>() + r0 : nullptr,
+          ignore, top_idx.data_ptr<int64_t>() + r0 * k,
+          stats.data_ptr<float>() + r0 * 2, ent.data_ptr<float>() + r0,
+          gp[0] ? gp[0] + r0 : nullptr, gp[1] ? gp[1] + r0 : nullptr,
+          gp[2] ? gp[2] + r0 * k : nullptr, n, (int)C, (int)k, (int)tile_rows,
+          (int)col_tiles, magic, (T*)dz.data_ptr() + r0 * C);
+    });
   });
   DOA_CHECK_HIP(hipGetLastError());
   return dz;

@@ -24,6 +24,9 @@ __device__ inline void wave_sync() {
 using Chunk = uint32_t __attribute__((ext_vector_type(4)));
 typedef Chunk LooseChunk __attribute__((aligned(2)));
 
+// a grid has fewer than 2^32 threads
+constexpr int64_t kMostThreads = ((int64_t)1 << 32) - 1024;
+
 inline hipStream_t stream_of_current() {
   return c10::hip::getCurrentHIPStream().stream();
 }

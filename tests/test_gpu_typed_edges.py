@@ -124,3 +124,54 @@ def test_no_slots(dev, groups, dtype):
         assert out.shape == (0, 4)
         dx, dw = torch.autograd.grad(out.sum(), (x, w))
         assert dx.shape == (0, 8) and not dw.any()
+
+
+def sliding(dev, rows, C, dtype=torch.bfloat16):
+    """rows x C logits, each row one element further on: no memory to speak of."""
+    line = torch.randn(rows + C, device=dev).to(dtype)
+    return line.as_strided((rows, C), (1, 1))
+
+
+def check_windows(z, t, k, marks, g=None):
+    """Rows around the marks are what a call of those rows alone gives."""
+    zr = z.detach().requires_grad_(g is not None)
+    a = ops.log_probs(zr, t, top_k=k)
+    dz = None
+    if g is not None:
+        dz, = torch.autograd.grad((a.log_prob, a.entropy), zr, g)
+    for m in marks:
+        at = slice(max(0, m - 20), min(z.shape[0], m + 20))
+        part = z[at].contiguous().requires_grad_(g is not None)
+        b = ops.log_probs(part, t[at], top_k=k)
+        for u, v in zip(a, b):
+            assert torch.equal(u[at], v), f"row {m}"
+        if g is not None:
+            d, = torch.autograd.grad((b.log_prob, b.entropy), part,
+                                     [v[at] for v in g])
+            assert torch.equal(dz[at], d), f"gradient of row {m}"
+
+
+@pytest.mark.parametrize("rows,C,k", [(2_150_000, 20000, 3),
+                                      (268_440_000, 257, 1)])
+def test_more_threads_than_one_grid(dev, rows, C, k):
+    """2^32 threads and more: a block of 1024 a part of a long row, sixteen lanes
+    a short one."""
+    lanes = 2 * 1024 if C == 20000 else 16
+    edge = (2 ** 32 - 1024) // lanes
+    assert rows > edge
+    z = sliding(dev, rows, C)
+    t = torch.randint(0, C, (rows,), device=dev)
+    check_windows(z, t, k, [0, rows // 3, edge - 10, edge, edge + 10, rows])
+    torch.cuda.empty_cache()
+
+
+def test_more_threads_than_one_grid_backward(dev):
+    """Two gradient tiles of 256 threads a row (and one block of 1024 forward)."""
+    rows, C = 8_390_000, 4097
+    back, front = (2 ** 32 - 1024) // 512, (2 ** 32 - 1024) // 1024
+    assert rows > back > front
+    z = sliding(dev, rows, C)
+    t = torch.randint(0, C, (rows,), device=dev)
+    g = [torch.randn(rows, device=dev) for _ in range(2)]
+    check_windows(z, t, 0, [0, front, back, rows // 3, rows], g)
+    torch.cuda.empty_cache()

@@ -687,44 +687,45 @@ __global__ __launch_bounds__(256) void sum_teams_kernel(
     const float* __restrict__ planes, ConstOffsets offsets, T* __restrict__ dw,
     int rows, int G, int64_t n, int teams) {
   __shared__ f32x4 part[4][64];
-  const int e = blockIdx.y;
-  const int b = offset_at(offsets, e, rows), s = offset_at(offsets, e + 1, rows);
   const Team tr = team_rows(offsets, rows, G, teams);
-  // (clamped for offsets that fall: the planes are never left)
-  const int t0 = min(teams - 1, max(0, b - tr.begin) / tr.each);
-  const int t1 = min(teams - 1, max(0, s - 1 - tr.begin) / tr.each);
-  if (s > b && t0 == t1) return;  // whole in one team
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const int many = s > b ? t1 - t0 + 1 : 0, each = (many + 3) >> 2;
-  const int from = t0 + min(many, wave * each);
-  const int to = t0 + min(many, wave * each + each);
-  for (int64_t i0 = (int64_t)blockIdx.x * 256; i0 < n;
-       i0 += (int64_t)gridDim.x * 256) {
-    const int64_t i = i0 + lane * 4;
-    const bool whole = n % 4 == 0;  // planes then start on 16 bytes
-    f32x4 sum = {};
-    if (i < n) {
+  for (int e = blockIdx.y; e < G; e += gridDim.y) {
+    const int b = offset_at(offsets, e, rows), s = offset_at(offsets, e + 1, rows);
+    // (clamped for offsets that fall: the planes are never left)
+    const int t0 = min(teams - 1, max(0, b - tr.begin) / tr.each);
+    const int t1 = min(teams - 1, max(0, s - 1 - tr.begin) / tr.each);
+    if (s > b && t0 == t1) continue;  // whole in one team
+    const int many = s > b ? t1 - t0 + 1 : 0, each = (many + 3) >> 2;
+    const int from = t0 + min(many, wave * each);
+    const int to = t0 + min(many, wave * each + each);
+    for (int64_t i0 = (int64_t)blockIdx.x * 256; i0 < n;
+         i0 += (int64_t)gridDim.x * 256) {
+      const int64_t i = i0 + lane * 4;
+      const bool whole = n % 4 == 0;  // planes then start on 16 bytes
+      f32x4 sum = {};
+      if (i < n) {
 #pragma unroll 8
-      for (int t = from; t < to; ++t) {
-        const float* p = planes + (2 * (int64_t)t + (t == t0)) * n + i;
-        if (whole) {
-          sum += *reinterpret_cast<const f32x4*>(p);
-        } else {
+        for (int t = from; t < to; ++t) {
+          const float* p = planes + (2 * (int64_t)t + (t == t0)) * n + i;
+          if (whole) {
+            sum += *reinterpret_cast<const f32x4*>(p);
+          } else {
 #pragma unroll
-          for (int r = 0; r < 4; ++r)
-            if (i + r < n) sum[r] += p[r];
+            for (int r = 0; r < 4; ++r)
+              if (i + r < n) sum[r] += p[r];
+          }
         }
       }
-    }
-    part[wave][lane] = sum;
-    __syncthreads();
-    if (wave == 0 && i < n) {
-      sum = ((part[0][lane] + part[1][lane]) + part[2][lane]) + part[3][lane];
+      part[wave][lane] = sum;
+      __syncthreads();
+      if (wave == 0 && i < n) {
+        sum = ((part[0][lane] + part[1][lane]) + part[2][lane]) + part[3][lane];
 #pragma unroll
-      for (int r = 0; r < 4; ++r)
-        if (i + r < n) dw[e * n + i + r] = (T)sum[r];
+        for (int r = 0; r < 4; ++r)
+          if (i + r < n) dw[e * n + i + r] = (T)sum[r];
+      }
+      __syncthreads();
     }
-    __syncthreads();
   }
 }
 
@@ -799,7 +800,7 @@ static void check_offsets(const at::Tensor& offsets, const at::Tensor& x,
                   offsets.is_contiguous() && offsets.numel() == groups + 1 &&
                   offsets.device() == x.device() && groups >= 1,
               what, ": int64 offsets [groups + 1] on the rows' device expected");
-  TORCH_CHECK(groups <= 65535, what, ": at most 65535 groups");
+  TORCH_CHECK(groups < (1 << 30), what, ": too many groups");
 }
 
 // blocks of a kernel that fills the chip once: a multiple of the 8 XCDs
@@ -940,7 +941,8 @@ at::Tensor segment_mm_wgrad(at::Tensor offsets, at::Tensor x, at::Tensor grad) {
                          planes.data_ptr<float>(), (int)R, (int)G, (int)K,
                          (int)N, (int)ceil_div(N, BN), (int)tiles, teams);
       hipLaunchKernelGGL((sum_teams_kernel<T>),
-                         dim3(grid_for(K * N, 256, 4096), G),
+                         dim3(grid_for(K * N, 256, 4096),
+                              (unsigned)std::min<int64_t>(G, 1024)),
                          dim3(256), 0, stream, planes.data_ptr<float>(), op,
                          (T*)dw.data_ptr(), (int)R, (int)G, K * N, teams);
     };

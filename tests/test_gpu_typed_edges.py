@@ -7,6 +7,7 @@ import pytest
 import torch
 
 import typed_oracle as oracle
+from test_gpu_typed_variants import check_mm
 from test_typed_ops import check_log_probs
 
 from dgl_operator_amd import ops
@@ -175,3 +176,47 @@ def test_more_threads_than_one_grid_backward(dev):
     g = [torch.randn(rows, device=dev) for _ in range(2)]
     check_windows(z, t, 0, [0, front, back, rows // 3, rows], g)
     torch.cuda.empty_cache()
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_more_groups_than_a_grid_is_high(dev, dtype):
+    """70000 groups of a row or so, and none in some."""
+    G, K, N = 70_000, 8, 12
+    gen = torch.Generator().manual_seed(1)
+    sizes = torch.randint(0, 3, (G,), generator=gen)
+    offsets = torch.cat((torch.zeros(1).long(), sizes.cumsum(0))).to(dev)
+    rows = int(offsets[-1])
+    group = torch.repeat_interleave(torch.arange(G), sizes).to(dev)
+    x = torch.randn(rows, K, device=dev).to(dtype).requires_grad_()
+    w = torch.randn(G, K, N, device=dev).to(dtype).requires_grad_()
+    g = torch.randn(rows, N, device=dev).to(dtype)
+    y = ops.segment_mm(offsets, x, w)
+    dx, dw = torch.autograd.grad(y, (x, w), g)
+    xw, gw, ww = x.detach().double(), g.double(), w.detach().double()[group]
+
+    def close(got, terms, steps):
+        ref, size = terms.sum(-1), terms.abs().sum(-1)
+        acc = 2 * (steps + 2) * oracle.U * size
+        tol = acc + oracle.half(dtype) * (ref.abs() + acc) + oracle.tiny(dtype)
+        assert ((got.detach().double() - ref).abs() <= tol).all()
+
+    close(y, xw[:, None, :] * ww.transpose(1, 2), K)
+    close(dx, gw[:, None, :] * ww, N)
+    outer = xw[:, :, None] * gw[:, None, :]
+    ref = torch.zeros(G, K, N, dtype=torch.float64, device=dev)
+    size = ref.index_add(0, group, outer.abs())
+    ref.index_add_(0, group, outer)
+    tol = 8 * oracle.U * size + oracle.half(dtype) * ref.abs() * 1.01 \
+        + oracle.tiny(dtype)
+    assert ((dw.double() - ref).abs() <= tol).all()
+
+
+@pytest.mark.parametrize("dtype,K,N", [(torch.float32, 16, 16),
+                                       (torch.bfloat16, 128, 136)])
+def test_many_groups_by_teams(dev, dtype, K, N):
+    """More groups than the teams' sums have rows of blocks."""
+    G = 1100
+    mean = 256 if dtype == torch.float32 else 512
+    sizes = [0 if e % 9 == 0 else mean + mean * (e % 5) // 4 for e in range(G)]
+    assert sum(sizes) >= mean * G
+    check_mm(dev, sizes, K, N, 0, 0, dtype, "plain")

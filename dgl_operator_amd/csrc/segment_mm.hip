@@ -847,8 +847,8 @@ at::Tensor segment_mm(at::Tensor offsets, at::Tensor x, at::Tensor weight,
   const int64_t R = x.size(0);
   TORCH_CHECK(R < (1 << 30), "segment_mm: too many rows");
   const auto op = (ConstOffsets)offsets.data_ptr<int64_t>();
-  auto y = at::empty({R, N}, x.options());
-  if (R * N == 0) return y;
+  if (R * N == 0) return at::empty({R, N}, x.options());
+  at::Tensor y;
   // one of the weight's two inner strides has to be 1
   const bool n_inner = N <= 1 ? wt.stride(1) != 1 || K <= 1 : wt.stride(2) == 1;
   if (!n_inner && !(K <= 1 || wt.stride(1) == 1)) wt = wt.contiguous();
@@ -857,7 +857,8 @@ at::Tensor segment_mm(at::Tensor offsets, at::Tensor x, at::Tensor weight,
   DOA_FLOAT_TYPES(x.scalar_type(), "segment_mm", [&] {
     auto go = [&](auto kernel, int BM, int BN, int threads) {
       const int64_t tn = ceil_div(N, BN), blocks = (R / BM + G) * tn;
-      TORCH_CHECK(blocks < INT32_MAX, "segment_mm: too many tiles");
+      TORCH_CHECK(blocks <= kMostThreads / threads, "segment_mm: too many tiles");
+      y = at::empty({R, N}, x.options());
       hipLaunchKernelGGL(kernel, dim3(blocks), dim3(threads), 0,
                          stream_of_current(), (const T*)xc.data_ptr(),
                          xc.stride(0), (const T*)wt.data_ptr(), wt.stride(0),
@@ -873,6 +874,7 @@ at::Tensor segment_mm(at::Tensor offsets, at::Tensor x, at::Tensor weight,
         if (N >= 256 && R >= 512 * G && K > 0) {
           const int64_t tn = ceil_div(N, 256), tiles = (R / 256 + G) * tn;
           TORCH_CHECK(tiles < (1 << 30), "segment_mm: too many tiles");
+          y = at::empty({R, N}, x.options());
           hipLaunchKernelGGL((segment_mm_wide_kernel<T, WC>), dim3(cu_count()),
                              dim3(512), 0, stream_of_current(),
                              (const T*)xc.data_ptr(), xc.stride(0),
@@ -923,8 +925,8 @@ at::Tensor segment_mm_wgrad(at::Tensor offsets, at::Tensor x, at::Tensor grad) {
   auto gc = mm_rows(grad);
   const int64_t K = x.size(1), N = grad.size(1), R = x.size(0);
   TORCH_CHECK(R < (1 << 30), "segment_mm: too many rows");
-  auto dw = at::empty({G, K, N}, x.options());
-  if (dw.numel() == 0) return dw;
+  if (G * K * N == 0) return at::empty({G, K, N}, x.options());
+  at::Tensor dw;
   DOA_FLOAT_TYPES(x.scalar_type(), "segment_mm", [&] {
     const bool whole = whole_rows<T>(xc, K) && whole_rows<T>(gc, N);
     const T* xp = (const T*)xc.data_ptr();
@@ -935,6 +937,7 @@ at::Tensor segment_mm_wgrad(at::Tensor offsets, at::Tensor x, at::Tensor grad) {
     at::Tensor planes;
     auto by_teams = [&](auto kernel, int blocks, int threads, int BN,
                         int64_t tiles, int teams) {
+      dw = at::empty({G, K, N}, x.options());
       planes = at::empty({2 * teams * K * N}, x.options().dtype(at::kFloat));
       hipLaunchKernelGGL(kernel, dim3(blocks), dim3(threads), 0, stream, xp,
                          xc.stride(0), gp, gc.stride(0), op, (T*)dw.data_ptr(),
@@ -974,7 +977,8 @@ at::Tensor segment_mm_wgrad(at::Tensor offsets, at::Tensor x, at::Tensor grad) {
                  (int)(teams * tiles), 256, B, tiles, (int)teams);
         return;
       }
-      TORCH_CHECK(tiles * G < INT32_MAX, "segment_mm: too many tiles");
+      TORCH_CHECK(tiles <= kMostThreads / 256 / G, "segment_mm: too many tiles");
+      dw = at::empty({G, K, N}, x.options());
       auto go = [&](auto kernel) {
         hipLaunchKernelGGL(kernel, dim3(tiles * G), dim3(256), 0, stream, xp,
                            xc.stride(0), gp, gc.stride(0), op,

@@ -64,7 +64,9 @@ def segment_mm(offsets: torch.Tensor, x: torch.Tensor,
              [groups, N, K] is read in place)
 
     Groups may be empty; rows of no group give zeros. Products accumulate in
-    fp32 and are rounded once. Gradients reach x and weight.
+    fp32 and are rounded once. Gradients reach x and weight. On GPU rows, K and N
+    are below 2^30, and what would take more blocks than one launch holds (16
+    million tiles of at least 32 x 64) is refused.
     """
     assert offsets.dim() == 1 and offsets.dtype == torch.int64, \
         "segment_mm: int64 offsets [groups + 1] expected"

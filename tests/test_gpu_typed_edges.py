@@ -220,3 +220,21 @@ def test_many_groups_by_teams(dev, dtype, K, N):
     sizes = [0 if e % 9 == 0 else mean + mean * (e % 5) // 4 for e in range(G)]
     assert sum(sizes) >= mean * G
     check_mm(dev, sizes, K, N, 0, 0, dtype, "plain")
+
+
+def test_more_tiles_than_one_launch_holds(dev):
+    """Refused before anything is allocated or launched."""
+    rows = 2 ** 30 - 1
+    x = torch.ones(1, 1, device=dev).expand(rows, 1)
+    w = torch.ones(1, 1, 65, device=dev)
+    offsets = torch.tensor([0, rows], device=dev)
+    with pytest.raises(RuntimeError, match="too many tiles"):
+        ops.segment_mm(offsets, x, w)
+    G = 4_200_000
+    w = torch.ones(1, 65, 65, device=dev).expand(G, 65, 65).requires_grad_()
+    offsets = torch.ones(G + 1, dtype=torch.int64, device=dev)
+    offsets[0] = 0
+    y = ops.segment_mm(offsets, torch.ones(1, 65, device=dev), w)
+    assert torch.equal(y, torch.full_like(y, 65.0))
+    with pytest.raises(RuntimeError, match="too many tiles"):
+        torch.autograd.grad(y.sum(), w)

@@ -31,6 +31,10 @@ def _edge_dst(indptr: torch.Tensor) -> torch.Tensor:
     )
 
 
+# elements of the messages that the CPU path holds at a time
+_REF_ELEMENTS = 1 << 20
+
+
 def _spmm_ref(
     indptr: torch.Tensor,
     indices: torch.Tensor,
@@ -40,15 +44,21 @@ def _spmm_ref(
 ) -> torch.Tensor:
     """CPU reference: out[v] = reduce over positions p in [indptr[v], indptr[v+1])."""
     num_rows = indptr.numel() - 1
-    msg = feat[indices]
-    if eweight is not None:
-        msg = msg * eweight.unsqueeze(-1)
     # hub rows sum thousands of messages one after the other: in 32 bits the
-    # rounding alone passes 1e-4 (1.15e-4 over 7388 in-edges), so sum in 64
+    # rounding alone passes 1e-4 (1.15e-4 over 7388 in-edges), so sum in 64, a
+    # stretch of edges at a time: all messages at once would take their memory
+    # twice more
     out = torch.zeros(
         (num_rows,) + feat.shape[1:], dtype=torch.float64, device=feat.device
     )
-    out.index_add_(0, _edge_dst(indptr), msg.double())
+    dst = _edge_dst(indptr)
+    step = max(1, _REF_ELEMENTS // max(1, feat[:1].numel()))
+    for start in range(0, indices.numel(), step):
+        part = slice(start, start + step)
+        msg = feat[indices[part]]
+        if eweight is not None:
+            msg = msg * eweight[part].unsqueeze(-1)
+        out.index_add_(0, dst[part], msg.double())
     if mean:
         deg = (indptr[1:] - indptr[:-1]).clamp(min=1).double()
         out = out / deg.view(-1, *([1] * (feat.dim() - 1)))

@@ -437,6 +437,9 @@ static void check_rows(const at::Tensor& t, const at::Tensor& position,
   TORCH_CHECK(t.is_cuda() && t.device() == position.device() && t.dim() == 2 &&
                   t.size(0) == rows,
               what, ": [", rows, ", D] rows on the plan's device expected");
+  // columns are counted in 32 bits, a wave's step beyond the last one too
+  TORCH_CHECK(t.size(1) < (1 << 30), what, ": rows of fewer than 2^30 elements "
+              "expected, got ", t.size(1));
 }
 
 static const float* weights_ptr(const c10::optional<at::Tensor>& w,

@@ -140,7 +140,7 @@ class _CombineRows(torch.autograd.Function):
 def dispatch_rows(route: RowRoute, x: torch.Tensor) -> torch.Tensor:
     """x [rows, ...] -> sorted rows [rows * k, ...]: row ``route.position[t, j]``
     is x[t]; rows behind the last group are zero. Its gradient sums the copies
-    of each row."""
+    of each row. On GPU a row has fewer than 2^30 elements."""
     rows, k = route.position.shape
     assert x.dim() >= 2 and x.shape[0] == rows, \
         f"dispatch_rows: [{rows}, ...] rows expected, got {tuple(x.shape)}"
@@ -163,8 +163,9 @@ def combine_rows(
     """Sorted rows y [rows * k, ...] -> [rows, ...]:
     out[t] = sum_j weights[t, j] * y[route.position[t, j]], dropped slots adding
     nothing. weights is [rows, k] (any float type; all ones when None; [rows]
-    will do for k = 1). Sums are in 32 bits, rounded once; gradients reach y and
-    weights."""
+    will do for k = 1). Sums are in 32 bits, rounded once, on GPU with the weights
+    in 32 bits too; gradients reach y and weights. On GPU a row has fewer than
+    2^30 elements."""
     rows, k = route.position.shape
     assert y.dim() >= 2 and y.shape[0] == rows * k, \
         f"combine_rows: [{rows * k}, ...] rows expected, got {tuple(y.shape)}"

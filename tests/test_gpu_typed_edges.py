@@ -238,3 +238,19 @@ def test_more_tiles_than_one_launch_holds(dev):
     assert torch.equal(y, torch.full_like(y, 65.0))
     with pytest.raises(RuntimeError, match="too many tiles"):
         torch.autograd.grad(y.sum(), w)
+
+
+def test_rows_too_wide_are_refused(dev):
+    """Columns are counted in 32 bits: wider rows raise, nothing is left out."""
+    route = ops.route_rows(torch.zeros(1, dtype=torch.int64, device=dev), 1)
+    for width in (2 ** 30, 2 ** 31, 2 ** 32 + 8):
+        x = torch.ones(1, 1, dtype=torch.bfloat16, device=dev).expand(1, width)
+        with pytest.raises(RuntimeError, match="fewer than 2\\^30"):
+            ops.dispatch_rows(route, x)
+        with pytest.raises(RuntimeError, match="fewer than 2\\^30"):
+            ops.combine_rows(route, x)
+    x = torch.arange(2 ** 30 - 4, dtype=torch.int32, device=dev).to(torch.bfloat16)
+    out = ops.combine_rows(route, ops.dispatch_rows(route, x[None]))
+    assert torch.equal(out[0], x)
+    del x, out
+    torch.cuda.empty_cache()

@@ -64,8 +64,8 @@ def build(force: bool = False, verbose: bool = True) -> Path:
         "-fPIC",
         "-fno-gpu-rdc",
         "-munsafe-fp-atomics",
-        # some packed fp32 forms have given wrong results on these parts now
-        # and then: keep the compiler from making them
+        # no packed fp32 instructions: a precaution, some of their forms are
+        # not trusted on these parts
         "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops",
         "-D__HIP_PLATFORM_AMD__=1",
         "-DUSE_ROCM=1",

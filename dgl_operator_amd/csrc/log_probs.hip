@@ -10,11 +10,21 @@
 //
 // Order of the alternatives: by value, NaN first, equal values by index.
 //
-// Bound by memory where there is enough to read. Measured on one MI355X (a large
-// copy 4.8 TB/s): 2449029 x 47 in fp16 with the five best 112 us (3.7 TB/s; ~24
-// vector instructions a logit are 70 of them), 1024 x 14951 in bf16 with the ten
-// best 19 us and its gradient 20 us (the chain of one row's steps, twice a CU at a
-// time; 6 and 13 us of copying), 8 x 14951 in fp32 6.5 us, 1000 x 47 4 us.
+// e^x is 2^(x log2 e) with the product rounded to fp32: off by |x| 2^-24 of
+// itself, beside as much from the rounding of z - m, where its terms weigh e^-|x|.
+// expf left the results no nearer (entropies of 14951 classes within 1.3e-6 of 64
+// bits with both, fp32 gradients within 3.5e-8 of their size) and took longer:
+// 2449029 x 47 with the five best 135 us instead of 122, 4096 x 14951 53 instead
+// of 41, their gradients 153 instead of 135 and 59 instead of 51.
+//
+// Measured on one MI355X (a large copy 4.8 TB/s): 2449029 x 47 in fp16 with the
+// five best 114 us (91 of copying; ~24 vector instructions a logit are 70 of
+// them), 1024 x 14951 in bf16 with the ten best 17-20 us and its gradient 21 us
+// (the chain of one row's steps, twice a CU at a time; 6 and 13 us of copying),
+// 8 x 14951 in fp32 7 us, 1000 x 47 4.4 us. Further from the copy's time where
+// lanes keep long lists, 100000 x 100 with the ten best: bf16 26 us (7), fp32 65
+// (11); and where a row is short for its block, 20000 x 2000 in bf16 68 us (17),
+// 600 x 115412 in bf16 65 us (29).
 
 #include "vec.h"
 
@@ -753,7 +763,10 @@ log_probs_fwd(at::Tensor logits, c10::optional<at::Tensor> target, int64_t k,
               r.top_lp, r.top_idx, r.stats, wave_bytes);
         });
       };
-      auto slots = [&](auto lv) {  // registers for the next such number of keys
+      // Registers for the next such number of keys; each number is a kernel that
+      // takes long to compile. 2449029 x 47 in fp16: none 60 us, 1 71, 2 81, 5 115,
+      // 6 138, 10 239, 16 422, 32 998 (copying 61, 67, 73, 91, 97, 122, 159, 257).
+      auto slots = [&](auto lv) {
         if (k == 0) go(lv, std::integral_constant<int, 0>{});
         else if (k == 1) go(lv, std::integral_constant<int, 1>{});
         else if (k <= 5) go(lv, std::integral_constant<int, 5>{});

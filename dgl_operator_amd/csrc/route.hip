@@ -275,8 +275,8 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor> route_rows(at::Tensor ids,
 // The row kernels: 2^sh lanes a row, 16 bytes a lane where rows allow it.
 // Bound by memory. They go over the rows before sorting, so that each of those
 // is read (or written) once whatever k, and the sorted rows once each. 262144
-// rows of 512 in bf16 with k = 2: copy out 132 us (6.1 TB/s), weighted sum 157 us
-// (5.1 TB/s), its gradient 257 us (5.2 TB/s).
+// rows of 512 in bf16 with k = 2: copy out 137 us (5.9 TB/s), weighted sum 167 us
+// (4.8 TB/s), its gradient 263 us (5.1 TB/s).
 // ---------------------------------------------------------------------------
 
 // a slot's row: not that of a dropped one, and never outside the sorted rows

@@ -11,16 +11,19 @@
 // last, partial tile, so a block finds its group by a search of the offsets.
 //
 // Measured on one MI355X (a large copy 4.8 TB/s, a large bf16 product 1230 and
-// fp32 153 TFLOP/s):
-//   262144 rows, 8 x 512 x 1024, bf16   y 344, dx 317, dW 287 us (0.8, 0.87, 0.96
-//       PFLOP/s). The matrix instructions alone take 196 us, the loads alone
-//       189; 537 MB of y to write, and L2, keep the two from hiding each other
-//       whole. One weight for all rows in the library: y 358, dx 236 us.
-//   65536 rows, 1345 x 400 x 400, fp16   145, 146, 163 us: 430 MB of weights to
+// fp32 153 TFLOP/s), each product by itself, ten calls back to back:
+//   262144 rows, 8 x 512 x 1024, bf16   y 339, dx 304, dW 278 us (0.81, 0.90, 0.99
+//       PFLOP/s; the first calls after a pause 390, 360, 326). The matrix
+//       instructions alone take 196 us, the loads alone 189; 537 MB of y to
+//       write, and L2, keep the two from hiding each other whole. One weight for
+//       all rows in the library: y 358, dx 236 us.
+//   65536 rows, 1345 x 400 x 400, bf16   133, 142, 177 us: 430 MB of weights to
 //       read or write each time, 112 us of copying.
-//   53504 rows, 16 x 100 x 256, fp32    40, 42, 46 us against 18 of matrix rate;
+//   53504 rows, 16 x 100 x 256, fp32    39, 41, 49 us against 18 of matrix rate;
 //       partial tiles (100 of 112, groups' last rows) are a fifth, the first
 //       loads and the last blocks of so short a kernel most of the rest.
+//   186248 rows, 415 x 618 x 19, bf16 (unaligned)   106, 57, 147 us against 52 of
+//       copying: through registers, one step ahead.
 //   16 rows, 8 x 256 x 512, bf16   5 us, a few rows a group: latency.
 
 #include "vec.h"
@@ -438,8 +441,8 @@ __global__ __launch_bounds__(64 * WM * WN, WAVES) void segment_mm_kernel(
 // ---------------------------------------------------------------------------
 // Many rows a group, 16-bit types: one block of 8 waves a CU walks over tiles of
 // 256 x 256: a smaller tile asks more of L2 than it gives (128 x 128 is 64 bytes
-// a clock and CU at the matrix rate; measured y 437, dx 353 us where this is 352
-// and 315). Steps of 64 bytes of depth go round a ring of 4 LDS stages: one is
+// a clock and CU at the matrix rate; y 437 and dx 353 us in the run where this was
+// 352 and 315). Steps of 64 bytes of depth go round a ring of 4 LDS stages: one is
 // multiplied from registers while the next is read into them and three more are
 // on their way; the loads run on into the next tile while this one's results go
 // out.
@@ -884,11 +887,18 @@ at::Tensor segment_mm(at::Tensor offsets, at::Tensor x, at::Tensor weight,
           return;
         }
       }
-      // Few rows a group: a lower tile leaves less of it empty and reads the
-      // weights over more blocks. Above that, steps of 64 bytes let four blocks
-      // share a CU and hide each other's first loads and stores (400 x 400 for
-      // 1345 groups in bf16: 49 rows a group 133 us with 64 rows, 139 with 128;
-      // 195 rows a group 283 and 256, and 277 with steps of 128 bytes).
+      // Few rows a group: a lower tile leaves less of it empty and spreads the
+      // weights over more blocks; many: a higher one reads them less often. us
+      // with tiles of 32, 64 and (16-bit) 128 rows, by rows a group:
+      //   rows                   16            32            48            96
+      //   bf16 1345 x 400 x 400  110 111 116   130 121 127   157 132 139   241 178 175
+      //   bf16 256 x 512 x 512   26 27 32      27 28 32      31 28 34      44 35 35
+      //   fp32 1345 x 400 x 400  209 275       246 300       307 337       501 503
+      //   fp32 16 x 512 x 512    10 17         11 18         15 18         16 25
+      // 48 lies between where 16-bit products of many groups change (about 20)
+      // and fp32 ones (about 60). From 97 on (128 rows: 297 221 202, 54 41 37)
+      // steps of 64 bytes let four blocks share a CU and hide each other's first
+      // loads and stores (1345 groups of 195 rows 256 us, 277 with 128 bytes).
       if (R <= 48 * G)
         go(segment_mm_kernel<T, WC, W, 32, 64, 1, 4, 128, 2>, 32, 64, 256);
       else if constexpr (sizeof(T) == 4)

@@ -323,3 +323,70 @@ def test_no_rows(dev):
         assert a.top_index.shape == (0, 1)
         g, = torch.autograd.grad(a.log_prob.sum() + a.entropy.sum(), z)
         assert g.shape == z.shape
+
+
+# ---------------------------------------------------------------------------
+# the variants with workspaces, captured
+# ---------------------------------------------------------------------------
+def long_groups(dev):
+    """The tiled plan, 256 x 256 products and dW by teams."""
+    ids = torch.randint(-1, 6, (4400, 2), device=dev)
+    x = torch.randn(4400, 2048, device=dev).bfloat16()
+    w = (torch.randn(6, 2048, 2048, device=dev) / 45).bfloat16()
+
+    def step(ids, x, w):
+        route = ops.route_rows(ids, 6)
+        xs = ops.dispatch_rows(route, x)
+        y = ops.segment_mm(route.offsets, xs, w)
+        out = ops.combine_rows(route, y)
+        return (route.position, out) + torch.autograd.grad(
+            out, (x, w), torch.ones_like(out))
+
+    return [ids, x, w], step
+
+
+def long_rows(dev):
+    """Rows in parts that are joined."""
+    z = torch.randn(9, 40001, device=dev).half()
+    t = torch.randint(0, 40001, (9,), device=dev)
+
+    def step(t, z):
+        a = ops.log_probs(z, t, top_k=7)
+        g, = torch.autograd.grad(a.log_prob.sum() + a.entropy.sum(), z)
+        return a + (g,)
+
+    return [t, z], step
+
+
+@pytest.mark.parametrize("make", [long_groups, long_rows])
+def test_workspaces_in_two_graphs(dev, make):
+    """Two graphs of one program, replayed in turn with eager runs of it between
+    and new inputs each time, give what the eager runs give."""
+    ins, step = make(dev)
+
+    def run(ts):
+        return step(*[t.detach().requires_grad_(t.is_floating_point())
+                      for t in ts])
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        for _ in range(2):
+            run(ins)
+    torch.cuda.current_stream().wait_stream(side)
+    graphs = []
+    for _ in range(2):
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            outs = run(ins)
+        graphs.append((graph, outs))
+    for i in range(3):
+        ins[0].copy_(ins[0].flip(0))
+        ins[1].copy_(torch.randn(ins[1].shape, device=dev))
+        want = run([t.clone() for t in ins])
+        torch.cuda.synchronize()
+        for graph, outs in graphs:
+            graph.replay()
+            torch.cuda.synchronize()
+            for a, b in zip(outs, want):
+                assert torch.equal(a, b)
